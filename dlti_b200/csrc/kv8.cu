@@ -1,0 +1,643 @@
+// A paged cache of keys and values in 8 bits: rows written (dlti_rope_cache8, dlti_acc_rope_cache8), attention of single tokens over it
+// (dlti_paged_decode8), cached rows laid out in 16 bits (dlti_gather_rows8).
+//
+// Pages are [num_blocks, KV_heads, block_size, 128] e4m3: the tokens of one page and head are contiguous, so that attention reads whole
+// lines and a page's scale belongs to one piece of memory. Scales are [num_blocks, KV_heads] fp32, powers of two: e4m3 is a floating type, a
+// finer scale would not make its numbers more exact, and with a power of two a number leaves and enters without a second rounding.
+#include "common.cuh"
+
+#include <cstdio>
+
+namespace {
+
+constexpr int HD = 128;
+constexpr int E_LOW = -120, E_HIGH = 120;      // exponents of a page's scale: its reciprocal and 448 of it are normal fp32 numbers
+
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
+
+// Smallest power of two s with largest <= 448 s, 448 = 1.75 * 2^8.
+__device__ __forceinline__ float scale_for(float largest) {
+  const uint32_t u = __float_as_uint(largest);
+  const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u);
+  return pow2i(max(E_LOW, min(E_HIGH, e)));
+}
+// low byte of the result: a
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_of_e4m3x2(uint32_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
+  return r;
+}
+__device__ __forceinline__ float2 float2_of_e4m3x2(uint32_t v) {
+  const uint32_t h = half2_of_e4m3x2(v);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const int4& v, float (&f)[8]) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 t = Cvt<T>::unpack2(u[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ int4 pack8(const float (&f)[8]) {
+  int4 v;
+  uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = Cvt<T>::pack2(f[2 * i], f[2 * i + 1]);
+  return v;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Rows of a step. Sixteen lanes hold one head of one row, 8 elements each; the element that a rotation pairs with is 8 lanes away.
+// A warp takes the rows of one page (consecutive rows with slots in it) for one key or value head, so nobody else touches that head's piece
+// of the page or its scale. Query heads are only rotated: a warp takes up to 8 of a row.
+// ---------------------------------------------------------------------------------------------
+struct Rows8 {
+  const void* x;                 // [tokens, x_ld] in the rows' type, or the fp32 accumulator [tokens, (H + 2 KV) * 128], left zero
+  void* out;                     // [tokens, out_ld]; may be x
+  long long x_ld, out_ld;
+  const int* pos;
+  const float *cos_t, *sin_t;
+  const long long* slots;
+  uint8_t *k8, *v8;
+  float *ks, *vs;
+  int tokens, H, KV, bs;
+};
+
+template <typename T, bool ACC>
+__device__ __forceinline__ int4 take(const Rows8& p, long long t, int h, int l16) {
+  if constexpr (ACC) {
+    float4* a = reinterpret_cast<float4*>(const_cast<float*>(reinterpret_cast<const float*>(p.x)) + t * p.x_ld + h * HD + l16 * 8);
+    const float4 a0 = a[0], a1 = a[1];
+    a[0] = make_float4(0.f, 0.f, 0.f, 0.f);
+    a[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float r[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+    return pack8<T>(r);
+  } else {
+    return *reinterpret_cast<const int4*>(reinterpret_cast<const T*>(p.x) + t * p.x_ld + h * HD + l16 * 8);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void angles(const Rows8& p, long long t, int l16, float (&c)[8], float (&s)[8]) {
+  const long long at = (long long)p.pos[t] * (HD / 2) + (l16 & 7) * 8;
+  const float4 c0 = *reinterpret_cast<const float4*>(p.cos_t + at), c1 = *reinterpret_cast<const float4*>(p.cos_t + at + 4);
+  const float4 s0 = *reinterpret_cast<const float4*>(p.sin_t + at), s1 = *reinterpret_cast<const float4*>(p.sin_t + at + 4);
+  const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    c[j] = Cvt<T>::to_f(Cvt<T>::from_f(cc[j]));
+    const float v = Cvt<T>::to_f(Cvt<T>::from_f(ss[j]));
+    s[j] = l16 < 8 ? -v : v;
+  }
+}
+// The lane's 8 elements rotated (all lanes of the warp call). Products of two 16-bit numbers are exact in fp32, so one rounding is left.
+template <typename T>
+__device__ __forceinline__ int4 turn(const int4& v, const float (&c)[8], const float (&s)[8]) {
+  int4 w;
+  w.x = __shfl_xor_sync(0xffffffffu, v.x, 8);
+  w.y = __shfl_xor_sync(0xffffffffu, v.y, 8);
+  w.z = __shfl_xor_sync(0xffffffffu, v.z, 8);
+  w.w = __shfl_xor_sync(0xffffffffu, v.w, 8);
+  float a[8], b[8];
+  unpack8<T>(v, a);
+  unpack8<T>(w, b);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = a[j] * c[j] + b[j] * s[j];
+  return pack8<T>(a);
+}
+
+constexpr int KEEP = 8;          // pairs of rows that a warp keeps in registers between finding the scale and rounding to it
+
+template <typename T, bool ACC>
+__global__ void __launch_bounds__(256) rows8_kernel(const Rows8 p, int block, int q_units) {
+  griddep_pass(p.tokens);
+  const int lane = threadIdx.x & 31, l16 = lane & 15, half = lane >> 4;
+  const int blocks = (p.tokens + block - 1) / block;
+  const long long kv_units = (long long)blocks * 2 * p.KV;
+  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const bool copy = ACC || p.out != p.x;
+  T* out = reinterpret_cast<T*>(p.out);
+  if (unit >= kv_units) {                                   // rotate up to 8 query heads of a row
+    const long long u = unit - kv_units;
+    const long long t = u / q_units;
+    if (t >= p.tokens) return;
+    const int h0 = (int)(u - t * q_units) * 8 + half;
+    int4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (h0 + 2 * i < p.H) v[i] = take<T, ACC>(p, t, h0 + 2 * i, l16);
+      else v[i] = make_int4(0, 0, 0, 0);
+    float c[8], s[8];
+    angles<T>(p, t, l16, c, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int4 r = turn<T>(v[i], c, s);
+      if (h0 + 2 * i < p.H) *reinterpret_cast<int4*>(out + t * p.out_ld + (h0 + 2 * i) * HD + l16 * 8) = r;
+    }
+    return;
+  }
+  const int hh = (int)(unit % (2 * p.KV));                  // key heads, then value heads
+  const bool key = hh < p.KV;
+  const int head = key ? hh : hh - p.KV;
+  const int col = p.H + hh;
+  uint8_t* cache = key ? p.k8 : p.v8;
+  float* scales = key ? p.ks : p.vs;
+  const int first = (int)(unit / (2 * p.KV)) * block, last = min(p.tokens, first + block);
+  auto page_of = [&](int t) { const long long s = p.slots[t]; return s < 0 ? -1 : (int)((uint32_t)s / (uint32_t)p.bs); };
+  for (int t = first; t < last;) {
+    const int page = page_of(t);
+    if (page >= 0 && t == first && t > 0 && page_of(t - 1) == page) {   // these rows belong to the warp of the rows before
+      while (t < last && page_of(t) == page) ++t;
+      continue;
+    }
+    // the run [t, t + n) of rows of this page; a row without a slot is by itself
+    int n = 1;
+    bool fresh = false;
+    if (page >= 0) {
+      fresh = (uint32_t)p.slots[t] % (uint32_t)p.bs == 0;
+      for (;;) {
+        const int r = t + n + lane;
+        const long long s = r < p.tokens ? p.slots[r] : -1;
+        const bool in = s >= 0 && (int)((uint32_t)s / (uint32_t)p.bs) == page;
+        const uint32_t out_of = ~__ballot_sync(0xffffffffu, in);
+        const int more = out_of ? __ffs(out_of) - 1 : 32;
+        fresh |= __any_sync(0xffffffffu, in && lane < more && (uint32_t)s % (uint32_t)p.bs == 0);
+        n += more;
+        if (more < 32) break;
+      }
+    }
+    int4 held[KEEP];
+    float largest = 0.f;
+    auto see = [&](int r, bool keep, int i) {
+      const bool ok = r < n;
+      const long long row = t + (ok ? r : 0);
+      int4 v = make_int4(0, 0, 0, 0);
+      if (ok) v = take<T, ACC>(p, row, col, l16);
+      if (key) {
+        float c[8], s[8];
+        angles<T>(p, row, l16, c, s);
+        v = turn<T>(v, c, s);
+      }
+      if (ok && (key || copy)) *reinterpret_cast<int4*>(out + row * p.out_ld + col * HD + l16 * 8) = v;
+      float f[8];
+      unpack8<T>(v, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = fabsf(f[j]);
+        if (ok && a < INFINITY) largest = fmaxf(largest, a);          // neither infinities nor NaN set the scale
+      }
+      return v;
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (2 * i < n) held[i] = see(2 * i + half, true, i);
+    for (int r = 2 * KEEP; r < n; r += 2) see(r + half, false, 0);
+    if (page >= 0) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      const long long sc = (long long)page * p.KV + head;
+      uint8_t* piece = cache + sc * p.bs * HD;
+      const float old = fresh ? pow2i(E_LOW) : scales[sc];
+      const float now = fmaxf(old, scale_for(largest));
+      if (!fresh && now > old) {                            // what the page holds is rounded to the new scale
+        const float ratio = old / now;
+        for (int i = lane; i < p.bs * (HD / 16); i += 32) {
+          int4 v = reinterpret_cast<const int4*>(piece)[i];
+          uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 a = float2_of_e4m3x2(u[j] & 0xffffu), b = float2_of_e4m3x2(u[j] >> 16);
+            u[j] = e4m3x2(a.x * ratio, a.y * ratio) | e4m3x2(b.x * ratio, b.y * ratio) << 16;
+          }
+          reinterpret_cast<int4*>(piece)[i] = v;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) scales[sc] = now;
+      const float inv = 1.f / now;
+      auto put = [&](int r, const int4& v) {
+        if (r >= n) return;
+        float f[8];
+        unpack8<T>(v, f);
+        uint2 o;
+        o.x = e4m3x2(f[0] * inv, f[1] * inv) | e4m3x2(f[2] * inv, f[3] * inv) << 16;
+        o.y = e4m3x2(f[4] * inv, f[5] * inv) | e4m3x2(f[6] * inv, f[7] * inv) << 16;
+        const uint32_t off = (uint32_t)p.slots[t + r] % (uint32_t)p.bs;
+        *reinterpret_cast<uint2*>(piece + off * HD + l16 * 8) = o;
+      };
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i)
+        if (2 * i < n) put(2 * i + half, held[i]);
+      for (int r = 2 * KEEP + half; r < n; r += 2)          // longer pages: this lane wrote (or, without a copy, read) these pieces itself
+        put(r, *reinterpret_cast<const int4*>(out + (long long)(t + r) * p.out_ld + col * HD + l16 * 8));
+    }
+    t += n;
+  }
+}
+
+template <typename T, bool ACC>
+int rows8_t(const Rows8& p, cudaStream_t st) {
+  const int q_units = (p.H + 7) / 8;
+  // one row a warp while all of them fit the GPU at once (the rows of a decode step are pages of their own), else 16: most rows of a prompt
+  // belong to the warp of a row before
+  const int block = (long long)p.tokens * 2 * p.KV <= 148 * 64 ? 1 : 16;
+  const long long units = (long long)((p.tokens + block - 1) / block) * 2 * p.KV + (long long)p.tokens * q_units;
+  DLTI_CUDA_CHECK(dlti_launch_pdl(p.tokens, rows8_kernel<T, ACC>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, st, p, block, q_units));
+  dlti_count_launch();
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Attention of single tokens. A CTA takes one split of one sequence's context for up to 8 query heads of one key/value head; its warps take
+// tiles of 16 tokens in turn and never wait for one another before the end.
+//
+// Both products are m16n8k16 in fp16 with fp32 sums: e4m3 numbers are fp16 numbers. Neither operand passes through shared memory. The order
+// of the contraction is free as long as both operands agree, so a lane takes 16 consecutive bytes of a key (dimensions 64 i + 16 t ...) as its
+// share of four k-steps, and 16 consecutive bytes of four values (tokens 2t, 2t+1, 2t+8, 2t+9, dimensions 16 g ...) as the columns g of 16
+// n-tiles: bytes of neighbouring tokens are paired by a permute.
+//   queries: scaled by a power of two per head so that their 16 bits are fp16 numbers exactly (down to 2^-39 of the head's largest);
+//   weights p s_v: p <= 1 times the page's value scale over the largest seen so far, as fp16 hi + lo, rows g and g + 8 of the same product:
+//   22 bits, absolutely 2^-40 of the largest.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t word(const int4& v, int i) { return (uint32_t)(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w); }
+
+constexpr int NW = 4;            // warps of a CTA
+constexpr float P_UNIT = 32768.f;
+
+struct Tile {
+  int4 k[2][2], v[2][2];         // [half of 8 tokens][64 dimensions], [half][token of a pair]
+  float ks[2], vs[2];
+};
+
+struct Attend8 {
+  const void* q;
+  long long q_ld;
+  const uint8_t *k8, *v8;
+  const float *ks, *vs;
+  const int *tables, *ctx;
+  int max_blocks, bs, G, KV, splits;
+  float scale_log2;
+  float *part_o, *part_ml;       // [batch, heads, splits, 128], [..., 2]
+  void* out;
+  long long out_ld;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
+  griddep_pass(gridDim.z);
+  const int split = blockIdx.x, b = blockIdx.z;
+  const int groups = (p.G + 7) / 8;
+  const int kvh = blockIdx.y / groups, h0 = kvh * p.G + (blockIdx.y % groups) * 8;
+  const int nh = min(8, (kvh + 1) * p.G - h0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int ctx = min(p.ctx[b], p.max_blocks * p.bs);
+  const int tiles = (ctx + 15) / 16;
+  const int per = (tiles + p.splits - 1) / p.splits;
+  const int end = min(tiles, (split + 1) * per);
+  int tile = split * per + warp;
+
+  uint32_t aq[8][2];
+  float fq = 0.f;
+  {
+    float f[2][16], top = 0.f;
+    if (g < nh) {
+      const T* qp = reinterpret_cast<const T*>(p.q) + b * p.q_ld + (long long)(h0 + g) * HD + 16 * t;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float a[8];
+        unpack8<T>(*reinterpret_cast<const int4*>(qp + 64 * i), a);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[i][j] = a[j];
+        unpack8<T>(*reinterpret_cast<const int4*>(qp + 64 * i + 8), a);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[i][8 + j] = a[j];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(f[i][j]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f[i][j] = 0.f;
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = max(-100, min(127, (int)(__float_as_uint(top) >> 23) - 127));
+    const float up = pow2i(14 - e);
+    fq = p.scale_log2 * pow2i(e - 14);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        aq[4 * i + w][0] = Cvt<__half>::pack2(f[i][4 * w] * up, f[i][4 * w + 1] * up);
+        aq[4 * i + w][1] = Cvt<__half>::pack2(f[i][4 * w + 2] * up, f[i][4 * w + 3] * up);
+      }
+  }
+
+  const int* table = p.tables + (long long)b * p.max_blocks;
+  // pages of a tile's halves; a half that begins at or after the end has none
+  auto pages = [&](int at, int (&pg)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int tb = at * 16 + 8 * h;
+      pg[h] = at < end && tb < ctx ? table[(uint32_t)tb / (uint32_t)p.bs] : -1;
+    }
+  };
+  auto fetch = [&](int at, const int (&pg)[2], Tile& x) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (pg[h] >= 0) {
+        const long long sc = (long long)pg[h] * p.KV + kvh;
+        const uint32_t off = (uint32_t)(at * 16 + 8 * h) % (uint32_t)p.bs;
+        const long long base = (sc * p.bs + off) * HD;
+        const uint8_t* kp = p.k8 + base + g * HD + 16 * t;
+        const uint8_t* vp = p.v8 + base + 2 * t * HD + 16 * g;
+        x.k[h][0] = ld_nc_v4(kp);
+        x.k[h][1] = ld_nc_v4(kp + 64);
+        x.v[h][0] = ld_nc_v4(vp);
+        x.v[h][1] = ld_nc_v4(vp + HD);
+        x.ks[h] = p.ks[sc];
+        x.vs[h] = p.vs[sc];
+      } else {
+        x.k[h][0] = x.k[h][1] = x.v[h][0] = x.v[h][1] = make_int4(0, 0, 0, 0);
+        x.ks[h] = 1.f;
+        x.vs[h] = pow2i(E_LOW);
+      }
+    }
+  };
+
+  float m = -INFINITY, l = 0.f, vref = pow2i(E_LOW);
+  float o[16][4];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+
+  int pg[2];
+  Tile nx;
+  pages(tile, pg);
+  fetch(tile, pg, nx);
+  pages(tile + NW, pg);
+  for (; tile < end; tile += NW) {
+    Tile x = nx;
+    fetch(tile + NW, pg, nx);
+    pages(tile + 2 * NW, pg);
+    float z[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const uint32_t w = word(x.k[h][s >> 2], s & 3);
+        mma_f16(c, aq[s][0], 0u, aq[s][1], 0u, half2_of_e4m3x2(w & 0xffffu), half2_of_e4m3x2(w >> 16));
+      }
+      const float f = fq * x.ks[h];
+      z[h][0] = c[0] * f;
+      z[h][1] = c[1] * f;
+    }
+    const bool edge = tile * 16 + 16 > ctx;
+    if (edge) {                                            // tokens behind the end: no weight, and whatever the page holds there is no value
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (tile * 16 + 8 * h + 2 * t + i >= ctx) {
+            z[h][i] = -INFINITY;
+            x.v[h][i] = make_int4(0, 0, 0, 0);
+          }
+    }
+    float mx = fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float vnew = fmaxf(vref, fmaxf(x.vs[0], x.vs[1]));
+    if (__any_sync(0xffffffffu, mx > m) || vnew > vref) {
+      const float mn = fmaxf(m, mx);
+      const float a = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2f(m - mn);
+      l *= a;
+      const float ao = a * (vref / vnew);
+      m = mn;
+      vref = vnew;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        o[j][0] *= ao;
+        o[j][1] *= ao;
+        o[j][2] *= ao;
+        o[j][3] *= ao;
+      }
+    }
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float p0 = ex2f(z[h][0] - m), p1 = ex2f(z[h][1] - m);
+      if (edge) {                                          // m may be -inf itself
+        if (tile * 16 + 8 * h + 2 * t >= ctx) p0 = 0.f;
+        if (tile * 16 + 8 * h + 2 * t + 1 >= ctx) p1 = 0.f;
+      }
+      l += p0 + p1;
+      const float f = x.vs[h] / vref * P_UNIT;
+      const __half2 a = __floats2half2_rn(p0 * f, p1 * f);
+      const float2 r = __half22float2(a);
+      const __half2 c = __floats2half2_rn(p0 * f - r.x, p1 * f - r.y);
+      hi[h] = *reinterpret_cast<const uint32_t*>(&a);
+      lo[h] = *reinterpret_cast<const uint32_t*>(&c);
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      uint32_t e[2], f[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        e[h] = __byte_perm(word(x.v[h][0], w), word(x.v[h][1], w), 0x5140);
+        f[h] = __byte_perm(word(x.v[h][0], w), word(x.v[h][1], w), 0x7362);
+      }
+      mma_f16(o[4 * w], hi[0], lo[0], hi[1], lo[1], half2_of_e4m3x2(e[0] & 0xffffu), half2_of_e4m3x2(e[1] & 0xffffu));
+      mma_f16(o[4 * w + 1], hi[0], lo[0], hi[1], lo[1], half2_of_e4m3x2(e[0] >> 16), half2_of_e4m3x2(e[1] >> 16));
+      mma_f16(o[4 * w + 2], hi[0], lo[0], hi[1], lo[1], half2_of_e4m3x2(f[0] & 0xffffu), half2_of_e4m3x2(f[1] & 0xffffu));
+      mma_f16(o[4 * w + 3], hi[0], lo[0], hi[1], lo[1], half2_of_e4m3x2(f[0] >> 16), half2_of_e4m3x2(f[1] >> 16));
+    }
+  }
+
+  // join the warps: lane (g, t) holds dimensions 32 t .. 32 t + 31 of head g
+  constexpr int PITCH = HD + 4;
+  __shared__ float s_o[NW][8][PITCH];
+  __shared__ float s_m[NW][8], s_l[NW][8];
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  {
+    const float f = vref / P_UNIT;
+    float* d = &s_o[warp][g][32 * t];
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      *reinterpret_cast<float4*>(d + j) = make_float4((o[j][0] + o[j][2]) * f, (o[j + 1][0] + o[j + 1][2]) * f, (o[j + 2][0] + o[j + 2][2]) * f,
+                                                      (o[j + 3][0] + o[j + 3][2]) * f);
+      *reinterpret_cast<float4*>(d + 16 + j) = make_float4((o[j][1] + o[j][3]) * f, (o[j + 1][1] + o[j + 1][3]) * f,
+                                                           (o[j + 2][1] + o[j + 2][3]) * f, (o[j + 3][1] + o[j + 3][3]) * f);
+    }
+    if (t == 0) {
+      s_m[warp][g] = m;
+      s_l[warp][g] = l;
+    }
+  }
+  __syncthreads();
+  for (int h = 0; h < nh; ++h) {
+    float gm = s_m[0][h], gl = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 1; w < NW; ++w) gm = fmaxf(gm, s_m[w][h]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float mw = s_m[w][h], lw = s_l[w][h];
+      const float a = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2f(mw - gm);
+      gl += lw * a;
+      acc += s_o[w][h][threadIdx.x] * a;
+    }
+    const long long row = (long long)b * (p.G * p.KV) + h0 + h;
+    if (p.splits == 1) {
+      reinterpret_cast<T*>(p.out)[b * p.out_ld + (long long)(h0 + h) * HD + threadIdx.x] = Cvt<T>::from_f(gl == 0.f ? 0.f : acc / gl);
+    } else {
+      p.part_o[(row * p.splits + split) * HD + threadIdx.x] = acc;
+      if (threadIdx.x == 0) *reinterpret_cast<float2*>(p.part_ml + (row * p.splits + split) * 2) = make_float2(gm, gl);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(HD) join8_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, int splits,
+                                                   T* __restrict__ out, long long out_ld) {
+  griddep_pass(gridDim.y);
+  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
+  const long long at = ((long long)b * gridDim.x + h) * splits;
+  float gm = -INFINITY;
+  for (int s = 0; s < splits; ++s) gm = fmaxf(gm, part_ml[(at + s) * 2]);
+  float acc = 0.f, gl = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(part_ml + (at + s) * 2);
+    const float a = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2f(ml.x - gm);
+    gl += ml.y * a;
+    acc += part_o[(at + s) * HD + d] * a;
+  }
+  out[b * out_ld + (long long)h * HD + d] = Cvt<T>::from_f(gl == 0.f ? 0.f : acc / gl);
+}
+
+template <typename T>
+int attend8_t(const Attend8& p, int batch, cudaStream_t st) {
+  const int H = p.G * p.KV;
+  DLTI_CUDA_CHECK(dlti_launch_pdl(batch, attend8_kernel<T>, dim3(p.splits, p.KV * ((p.G + 7) / 8), batch), dim3(32 * NW), 0, st, p));
+  if (p.splits > 1)
+    DLTI_CUDA_CHECK(dlti_launch_pdl(batch, join8_kernel<T>, dim3(H, batch), dim3(HD), 0, st, (const float*)p.part_o, (const float*)p.part_ml,
+                                    p.splits, (T*)p.out, p.out_ld));
+  dlti_count_launch(p.splits > 1 ? 2 : 1);
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Cached rows in 16 bits: row rows[i] of ext gets the keys and values of slot slots[i] at its key and value columns. A thread takes 8 numbers.
+// ---------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) gather8_kernel(T* __restrict__ ext, long long ext_ld, const long long* __restrict__ rows,
+                                                      const long long* __restrict__ slots, const uint8_t* __restrict__ k8,
+                                                      const uint8_t* __restrict__ v8, const float* __restrict__ ks, const float* __restrict__ vs,
+                                                      long long n, int H, int KV, int bs) {
+  const long long total = n * 2 * KV * 16;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const int c = (int)(i & 15);
+    const long long u = i >> 4;
+    const long long r = u / (2 * KV);
+    const int hh = (int)(u - r * 2 * KV);
+    const bool key = hh < KV;
+    const uint32_t slot = (uint32_t)slots[r], page = slot / (uint32_t)bs, off = slot - page * bs;
+    const long long sc = (long long)page * KV + (key ? hh : hh - KV);
+    const uint2 v = *reinterpret_cast<const uint2*>((key ? k8 : v8) + (sc * bs + off) * HD + c * 8);
+    const float s = (key ? ks : vs)[sc];
+    const float2 a = float2_of_e4m3x2(v.x & 0xffffu), b = float2_of_e4m3x2(v.x >> 16), d = float2_of_e4m3x2(v.y & 0xffffu), e = float2_of_e4m3x2(v.y >> 16);
+    const float f[8] = {a.x * s, a.y * s, b.x * s, b.y * s, d.x * s, d.y * s, e.x * s, e.y * s};
+    *reinterpret_cast<int4*>(ext + rows[r] * ext_ld + (long long)(H + hh) * HD + c * 8) = pack8<T>(f);
+  }
+}
+
+bool sizes_ok(const char* what, int H, int KV, int hd, int bs) {
+  if (hd == HD && KV > 0 && H > 0 && H % KV == 0 && bs >= 8 && bs % 8 == 0) return true;
+  char msg[200];
+  std::snprintf(msg, sizeof msg, "%s: heads of 128, query heads a multiple of key/value heads, pages of a multiple of 8 tokens (got %d, %d / %d, %d)",
+                what, hd, H, KV, bs);
+  dlti_set_error(msg);
+  return false;
+}
+
+}  // namespace
+
+// Rows x [tokens, x_ld] -> out [tokens, out_ld] (may be x): queries and keys rotated, values as they are; keys and values of the rows with
+// slots[t] >= 0 also go to the 8-bit pages. Rows of one page are consecutive.
+DLTI_API int dlti_rope_cache8(const void* x, long long x_ld, void* out, long long out_ld, const int* pos, const float* cos_t, const float* sin_t,
+                              const long long* slots, void* k8, void* v8, float* ks, float* vs, long long tokens, int H, int KV, int hd, int bs,
+                              int dtype, cudaStream_t st) {
+  if (!sizes_ok("rope_cache8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
+  if (tokens <= 0) return 0;
+  if (tokens > 1 << 24) return DLTI_ERR_TOO_LARGE;
+  const Rows8 p{x, out, x_ld, out_ld, pos, cos_t, sin_t, slots, (uint8_t*)k8, (uint8_t*)v8, ks, vs, (int)tokens, H, KV, bs};
+  if (dtype == DLTI_BF16) return rows8_t<__nv_bfloat16, false>(p, st);
+  if (dtype == DLTI_FP16) return rows8_t<__half, false>(p, st);
+  return DLTI_ERR_UNSUPPORTED;
+}
+
+// The same from the fp32 accumulator [tokens, (H + 2 KV) * 128] of the decode GEMM, which is left zero.
+DLTI_API int dlti_acc_rope_cache8(float* acc, void* out, long long out_ld, const int* pos, const float* cos_t, const float* sin_t,
+                                  const long long* slots, void* k8, void* v8, float* ks, float* vs, long long tokens, int H, int KV, int hd,
+                                  int bs, int dtype, cudaStream_t st) {
+  if (!sizes_ok("acc_rope_cache8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
+  if (tokens <= 0) return 0;
+  if (tokens > 1 << 24) return DLTI_ERR_TOO_LARGE;
+  const Rows8 p{acc, out, (long long)(H + 2 * KV) * HD, out_ld, pos, cos_t, sin_t, slots, (uint8_t*)k8, (uint8_t*)v8, ks, vs, (int)tokens, H, KV, bs};
+  if (dtype == DLTI_BF16) return rows8_t<__nv_bfloat16, true>(p, st);
+  if (dtype == DLTI_FP16) return rows8_t<__half, true>(p, st);
+  return DLTI_ERR_UNSUPPORTED;
+}
+
+// floats of workspace that dlti_paged_decode8 needs with more than one split
+DLTI_API long long dlti_paged_decode8_floats(int batch, int H, int splits) { return splits > 1 ? (long long)batch * H * splits * (HD + 2) : 0; }
+
+// q [batch, q_ld] (head h at column h * 128) -> out [batch, out_ld]; contexts of 0 give zeros.
+DLTI_API int dlti_paged_decode8(const void* q, long long q_ld, const void* k8, const void* v8, const float* ks, const float* vs,
+                                const int* tables, int max_blocks, const int* ctx, int batch, int bs, int H, int KV, int hd, float scale,
+                                int splits, float* workspace, void* out, long long out_ld, int dtype, cudaStream_t st) {
+  if (!sizes_ok("paged_decode8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
+  if (batch <= 0) return 0;
+  if (batch > 65535 || splits < 1 || (splits > 1 && !workspace)) return DLTI_ERR_BAD_ARG;
+  const Attend8 p{q, q_ld, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, tables, ctx, max_blocks, bs, H / KV, KV, splits,
+                  scale * 1.4426950408889634f, workspace, workspace + (long long)batch * H * splits * HD, out, out_ld};
+  if (dtype == DLTI_BF16) return attend8_t<__nv_bfloat16>(p, batch, st);
+  if (dtype == DLTI_FP16) return attend8_t<__half>(p, batch, st);
+  return DLTI_ERR_UNSUPPORTED;
+}
+
+// ext [*, ext_ld]: columns H * 128 .. (H + 2 KV) * 128 of the rows rows[0 .. n) from the pages' slots slots[0 .. n).
+DLTI_API int dlti_gather_rows8(void* ext, long long ext_ld, const long long* rows, const long long* slots, const void* k8, const void* v8,
+                               const float* ks, const float* vs, long long n, int H, int KV, int hd, int bs, int dtype, cudaStream_t st) {
+  if (!sizes_ok("gather_rows8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
+  if (n <= 0) return 0;
+  const long long need = (n * 2 * KV * 16 + 255) / 256, cap = (long long)dlti_num_sms() * 64;
+  const unsigned grid = (unsigned)(need < cap ? need : cap);
+  if (dtype == DLTI_BF16)
+    gather8_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((__nv_bfloat16*)ext, ext_ld, rows, slots, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, n, H, KV, bs);
+  else if (dtype == DLTI_FP16)
+    gather8_kernel<__half><<<grid, 256, 0, st>>>((__half*)ext, ext_ld, rows, slots, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, n, H, KV, bs);
+  else
+    return DLTI_ERR_UNSUPPORTED;
+  dlti_count_launch();
+  return (int)cudaGetLastError();
+}

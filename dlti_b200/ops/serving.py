@@ -224,3 +224,71 @@ def sample(logits, temperature=None, top_k=None, top_p=None, seeds=None, step: i
                  _lib.ptr(top_p), _lib.ptr(seeds), int(step), _lib.ptr(out), _lib.ptr(lp),
                  _lib.dtype_code(logits.dtype), _lib.stream_ptr()), "sample")
     return out, lp
+
+
+def sample_given_ref(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    """(token ids int64 [B], log-probs fp32 [B]) in double precision."""
+    x = logits.double()
+    x = torch.where(torch.isnan(x), float("-inf"), x)
+    B, V = x.shape
+    top, first = x.max(-1, keepdim=True)
+    first = (x == top).long().argmax(-1)
+
+    def row(t, off):
+        return torch.full((B, 1), off, dtype=torch.float64, device=x.device) if t is None else t.double()[:, None]
+
+    t = row(temperature, 0.0)
+    drawn = (t > 0)[:, 0]
+    w = torch.where(x == top, 1.0, torch.exp((x - top) / torch.where(t > 0, t.clamp_min(1e-30), 1.0)).nan_to_num(0.0))
+    order = torch.sort(x, descending=True, stable=True).indices
+    d = w.gather(-1, order)
+    rank = torch.arange(V, device=x.device)
+    k = row(top_k, 0.0)
+    keep = rank < torch.where(k > 0, k, float(V))
+    run = torch.cumsum(d * keep, -1)
+    p = row(top_p, 1.0).clamp_min(0.0)
+    keep = keep & ((p >= 1) | (rank <= (run < p * run[:, -1:]).sum(-1, keepdim=True)))
+    keep = keep & (d >= row(min_p, 0.0).clamp_max(1.0))
+    kept = torch.zeros_like(w).scatter_(-1, order, d * keep)
+    run = torch.cumsum(kept, -1)
+    goal = torch.minimum(u.double()[:, None].clamp_min(0.0) * run[:, -1:], run[:, -1:] * (1 - 2.3e-16))
+    token = torch.where(drawn, ((run > goal) & (kept > 0)).long().argmax(-1), first)
+    lp = (x.gather(-1, token[:, None]) - top)[:, 0].nan_to_num(0.0) - torch.where(x == top, 1.0, torch.exp(x - top).nan_to_num(0.0)).sum(-1).log()
+    none = top[:, 0] == float("-inf")
+    return token.masked_fill(none, 0), lp.masked_fill(none, float("-inf")).float()
+
+
+def sample_given(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, want_logprob=False, out=None):
+    """Tokens drawn with given random numbers u (float64 [B], in [0, 1)): logits [B, V], V up to 262144 -> token ids int64 [B] (+ log-prob at
+    temperature 1). Per-row device tensors as in `sample`, and min_p fp32 (0 = off); None = greedy / off.
+
+    Weights are exp((x - max) / temperature). Of the tokens by descending logit, ties by ascending index, the first top_k are kept; of these the
+    fewest that hold top_p of their weight; of these the ones of at least min_p times the largest weight. The draw is the first token, by index, at
+    which the running sum of what is kept exceeds u times its sum. Temperature <= 0: the largest logit at its lowest index. NaN counts as -inf; a
+    row of nothing else gives token 0 and log-prob -inf. The same logits and numbers give the same tokens everywhere."""
+    B, V = logits.shape
+    if u.dtype != torch.float64 or u.shape != (B,) or not u.is_contiguous():
+        raise ValueError("sample_given: a float64 number for each row")
+    for name, t, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                        ("min_p", min_p, torch.float32)):
+        if t is not None and (t.dtype != dt or t.shape != (B,) or not t.is_contiguous()):
+            raise ValueError(f"sample_given: {name} is {dt} [{B}]")
+    if out is not None and (out.dtype != torch.int64 or out.shape != (B,) or not out.is_contiguous()):
+        raise ValueError(f"sample_given: out is int64 [{B}]")
+    if not 1 <= V <= 1 << 18:
+        raise ValueError(f"sample_given: rows of 1 to 262144 logits, got {V}")
+    if not _lib.use_native(logits):
+        tok, lp = sample_given_ref(logits, u, temperature, top_k, top_p, min_p)
+        return tok if out is None else out.copy_(tok), lp if want_logprob else None
+    if logits.stride(1) != 1:
+        raise ValueError("sample_given: a row's logits are consecutive")
+    d = torch.cuda.current_device()
+    if any(t is not None and (not t.is_cuda or t.device.index != d) for t in (logits, u, temperature, top_k, top_p, min_p, out)):
+        raise ValueError(f"sample_given: every tensor is on the current device, cuda:{d}")
+    if out is None:
+        out = torch.empty(B, dtype=torch.int64, device=logits.device)
+    lp = torch.empty(B, dtype=torch.float32, device=logits.device) if want_logprob else None
+    f = _lib.fn("dlti_sample_given", [_V, _L, _I, _I, _V, _V, _V, _V, _V, _V, _V, _I, _V])
+    _lib.check(f(_lib.ptr(logits), logits.stride(0), B, V, _lib.ptr(u), _lib.ptr(temperature), _lib.ptr(top_k), _lib.ptr(top_p), _lib.ptr(min_p),
+                 _lib.ptr(out), _lib.ptr(lp), _lib.dtype_code(logits.dtype), _lib.stream_ptr()), "sample_given")
+    return out, lp

@@ -352,6 +352,30 @@ int dlti_sample(const void* logits, long long ld, int batch, int V, const float*
                 const int* top_k, const float* top_p, const unsigned long long* seeds,
                 unsigned long long step, long long* out, float* out_logprob, int dtype,
                 dlti_stream_t stream);
+/* tokens from given numbers u in [0, 1): temperature, top-k, top-p of its weight, min-p, ties to the lowest index; any pointer of settings may
+ * be NULL (greedy / off). V <= 262144. csrc/sample.cu */
+int dlti_sample_given(const void* logits, long long ld, int batch, int V, const double* u, const float* temperature, const int* top_k,
+                      const float* top_p, const float* min_p, long long* out, float* out_logprob, int dtype, dlti_stream_t stream);
+/* Cache in 8 bits (csrc/kv8.cu): pages [num_blocks, KV, block_size, 128] e4m3 with scales [num_blocks, KV], powers of two. Rows of one page are
+ * consecutive, a slot occurs once (-1: none). A row at place 0 begins its page; any other may raise its scale. out may be x. */
+int dlti_rope_cache8(const void* x, long long x_ld, void* out, long long out_ld, const int* pos, const float* cos_t, const float* sin_t,
+                     const long long* slots, void* k8, void* v8, float* ks, float* vs, long long tokens, int H, int KV, int hd, int bs, int dtype,
+                     dlti_stream_t stream);
+/* the same from the fp32 accumulator [tokens, (H + 2 KV) * 128], left zero */
+int dlti_acc_rope_cache8(float* acc, void* out, long long out_ld, const int* pos, const float* cos_t, const float* sin_t,
+                         const long long* slots, void* k8, void* v8, float* ks, float* vs, long long tokens, int H, int KV, int hd, int bs,
+                         int dtype, dlti_stream_t stream);
+/* attention of single tokens; workspace: dlti_paged_decode8_floats, none for one split */
+long long dlti_paged_decode8_floats(int batch, int H, int splits);
+int dlti_paged_decode8(const void* q, long long q_ld, const void* k8, const void* v8, const float* ks, const float* vs, const int* tables,
+                       int max_blocks, const int* ctx, int batch, int bs, int H, int KV, int hd, float scale, int splits, float* workspace,
+                       void* out, long long out_ld, int dtype, dlti_stream_t stream);
+/* key and value columns of ext's rows rows[0..n) from the cached tokens at slots[0..n) */
+int dlti_gather_rows8(void* ext, long long ext_ld, const long long* rows, const long long* slots, const void* k8, const void* v8, const float* ks,
+                      const float* vs, long long n, int H, int KV, int hd, int bs, int dtype, dlti_stream_t stream);
+/* pages from[i] -> to[i] (host arrays) of every layer of every cache: csrc/pages.cu */
+int dlti_copy_pages(void* const* bases, const int* layers, const long long* layer_bytes, const long long* page_stride, const long long* page_bytes,
+                    int caches, const int* from, const int* to, int pairs, dlti_stream_t stream);
 /* out[t] = src[t] in [0, n) ? sampled[src[t]] : ids[t]: the input ids of a step that continues the step in flight */
 int dlti_feed_ids(const long long* ids, const int* src, const long long* sampled, int n, long long* out, long long rows,
                   dlti_stream_t stream);
