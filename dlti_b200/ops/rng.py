@@ -35,6 +35,15 @@ def philox4x32(c0, c1, c2, c3, k0, k1):
     return c0, c1, c2, c3
 
 
+def uniforms(seeds) -> np.ndarray:
+    """A number in [0, 1) of 53 bits for each 64-bit seed (float64): the first two words of Philox keyed by the seed."""
+    s = np.asarray(seeds, dtype=np.int64).astype(np.uint64)
+    z = np.zeros_like(s)
+    with np.errstate(over="ignore"):
+        a, b, _, _ = philox4x32(z, z, z, z + np.uint64(0x5A18), s & _MASK, s >> _S32)
+    return ((a >> np.uint64(5)).astype(np.float64) * 67108864.0 + (b >> np.uint64(6)).astype(np.float64)) / 9007199254740992.0
+
+
 def dropout_threshold(p: float) -> int:
     t = np.float32(p) * np.float32(4294967296.0)
     return int(min(np.float32(t), np.float32(4294967295.0)))

@@ -190,6 +190,9 @@ def sample_ref(logits, temperature, top_k, top_p, generator=None):
     return greedy, keep
 
 
+SAMPLE_MAX = 51200           # longest row of `sample` on a GPU (it is held in shared memory)
+
+
 def sample(logits, temperature=None, top_k=None, top_p=None, seeds=None, step: int = 0, want_logprob=False,
            out=None):
     """logits [B, V] -> token ids int64 [B] (+ log-prob at temperature 1). Per-row device tensors:

@@ -308,12 +308,19 @@ def start_frontend_process(eng: LLMEngine, host: str, port: int, model_name: str
 def _params_from_body(b: dict) -> SamplingParams:
     return SamplingParams(
         max_tokens=b.get("max_tokens", 16) or 16, temperature=float(b.get("temperature", 1.0) if b.get("temperature") is not None else 1.0),
-        top_p=float(b.get("top_p", 1.0) or 1.0), top_k=int(b.get("top_k", 0) or 0), n=int(b.get("n", 1) or 1),
+        top_p=float(b.get("top_p", 1.0) or 1.0), top_k=int(b.get("top_k", 0) or 0),
+        min_p=float(b.get("min_p", 0.0) or 0.0), n=int(b.get("n", 1) or 1),
         seed=b.get("seed"), stop=b.get("stop") or [], stop_token_ids=b.get("stop_token_ids") or [],
         ignore_eos=bool(b.get("ignore_eos", False)), min_tokens=int(b.get("min_tokens", 0) or 0),
         logprobs=b.get("logprobs"), echo=bool(b.get("echo", False)),
         skip_special_tokens=bool(b.get("skip_special_tokens", True)),
         detokenize=bool(b.get("detokenize", True)))
+
+
+def _answer(sp: SamplingParams, base_id: str, idx: int) -> SamplingParams:
+    """Parameters of answer idx of a request: n answers to each prompt follow one another, and all but the first may go on from its pages."""
+    first = idx // sp.n * sp.n
+    return SamplingParams(**{**vars(sp), "fork_of": None if idx == first else f"{base_id}-{first}"})
 
 
 def _error(message: str, typ: str = "invalid_request_error", code: int = 400):
@@ -429,7 +436,7 @@ def build_app(aeng: AsyncEngine, model_name: str):
                     rid = f"{base_id}-{idx}"
                     if sp.echo and isinstance(p, str):
                         await q.put(chunk(idx, p, None))
-                    async for item in aeng.generate(p, SamplingParams(**vars(sp)), rid):
+                    async for item in aeng.generate(p, _answer(sp, base_id, idx), rid):
                         if "error" in item:
                             await q.put({"error": {"message": item["error"], "type": "invalid_request_error", "param": None, "code": 400}})
                             break
@@ -463,7 +470,7 @@ def build_app(aeng: AsyncEngine, model_name: str):
         async def run_one(idx, p):
             rid = f"{base_id}-{idx}"
             text, lps, fin, pt, ct = (p if (sp.echo and isinstance(p, str)) else ""), [], None, 0, 0
-            async for item in aeng.generate(p, SamplingParams(**vars(sp)), rid):
+            async for item in aeng.generate(p, _answer(sp, base_id, idx), rid):
                 if "error" in item:
                     raise ValueError(item["error"])
                 text += item["text"]
@@ -523,7 +530,7 @@ def build_app(aeng: AsyncEngine, model_name: str):
                     rid = f"{base_id}-{idx}"
                     await q.put(obj("chat.completion.chunk", [{"index": idx, "delta": {"role": "assistant", "content": ""},
                                                                "finish_reason": None}]))
-                    async for item in aeng.generate(prompt, SamplingParams(**vars(sp)), rid):
+                    async for item in aeng.generate(prompt, _answer(sp, base_id, idx), rid):
                         if "error" in item:
                             await q.put({"error": {"message": item["error"], "type": "invalid_request_error", "param": None, "code": 400}})
                             break
@@ -556,7 +563,7 @@ def build_app(aeng: AsyncEngine, model_name: str):
 
         async def run_one(idx):
             text, fin, pt, ct = "", None, 0, 0
-            async for item in aeng.generate(prompt, SamplingParams(**vars(sp)), f"{base_id}-{idx}"):
+            async for item in aeng.generate(prompt, _answer(sp, base_id, idx), f"{base_id}-{idx}"):
                 if "error" in item:
                     raise ValueError(item["error"])
                 text += item["text"]

@@ -22,8 +22,9 @@ import torch
 
 from ..models.config import LlamaConfig
 from ..ops import serving as S
+from ..ops.rng import uniforms
 from ..models.registry import family_of
-from .kv_cache import BlockManager, KVCache, SlotManager, StateCache
+from .kv_cache import BlockManager, KVCache, KVCache8, SlotManager, StateCache
 from .model_runner import TPContext, TPWeights
 from .params import Request, SamplingParams, StepOutput
 from .scheduler import Batch, Scheduler
@@ -42,17 +43,17 @@ class StepLayout:
 
     `full` (runners with per_sequence = True): ctx, tables and the recurrent-state slots sslot cover the prompts
     too, rseq[T] names each row's sequence, and segs holds chunk_pieces of every kind of attention (nsg entries)."""
-    _I64 = ("ids", "slots", "last", "seeds", "pslots", "pdst", "csrc")
-    _I32 = ("pos", "src", "ctx", "cu", "ecu", "sslot", "rseq", "segs", "topk", "temp", "topp", "tables")
+    _I64 = ("ids", "slots", "last", "seeds", "unif", "pslots", "pdst", "csrc")
+    _I32 = ("pos", "src", "ctx", "cu", "ecu", "sslot", "rseq", "segs", "topk", "temp", "topp", "minp", "tables")
 
     def __init__(self, T: int, nd: int, npf: int, mb: int, ns: int | None = None, P: int = 0, full: bool = False,
-                 nsg: int = 0, nl: int | None = None):
+                 nsg: int = 0, nl: int | None = None, given: bool = False):
         """ns: prompts that are sampled in this step (default: all npf; fewer under chunked prefill, where a
         prompt's earlier chunks only fill the cache). P > 0: some prompt rows continue a prompt whose first P
         tokens (over all such prompts) are already in the paged cache: pslots[P] = their cache slots,
         pdst[P] / csrc[T - nd] = where prefix tokens / this step's prompt rows sit in the extended
         [prefix | chunk] attention layout, ecu[npf + 1] = its sequence boundaries. nl: rows whose logits are wanted
-        when that is not one per sampled sequence."""
+        when that is not one per sampled sequence. given: the step brings the random numbers that its tokens are drawn with (unif) and min-p."""
         ns = npf if ns is None else ns
         self.T, self.nd, self.npf, self.mb, self.ns, self.P = T, nd, npf, mb, ns, P
         B = nd + ns
@@ -60,26 +61,34 @@ class StepLayout:
         self.n = dict(ids=T, slots=T, last=B if nl is None else nl, seeds=B, pslots=P, pdst=P, csrc=(T - nd) if P else 0,
                       pos=T, src=T, ctx=nt, cu=npf + 1 if npf else 0, ecu=npf + 1 if P else 0, sslot=nt if full else 0,
                       rseq=T if full else 0, segs=nsg, topk=B, temp=B, topp=B, tables=nt * mb)
+        self.given = given
+        if given:
+            self.n.update(unif=B, minp=B)
         o = 0
         self.off = {}
-        for k in self._I64:
+        for k in self._sections(self._I64):
             self.off[k] = o
             o += self.n[k]
-        for k in self._I32:
+        for k in self._sections(self._I32):
             self.off[k] = o
             o += (self.n[k] + 1) // 2
         self.words = o
         self.tables = self.off["tables"]
 
+    def _sections(self, names):
+        return [k for k in names if k in self.n]
+
     def views(self, buf, xp) -> dict:
         """Typed views into `buf` (1-D int64 numpy array or torch tensor; xp = numpy or torch module)."""
-        i32, f32 = (np.int32, np.float32) if xp is np else (torch.int32, torch.float32)
+        i32, f32, f64 = (np.int32, np.float32, np.float64) if xp is np else (torch.int32, torch.float32, torch.float64)
         out = {}
-        for k in self._I64:
+        for k in self._sections(self._I64):
             out[k] = buf[self.off[k]:self.off[k] + self.n[k]]
-        for k in self._I32:
+        if self.given:
+            out["unif"] = out["unif"].view(f64)
+        for k in self._sections(self._I32):
             n = self.n[k]
-            out[k] = buf[self.off[k]:self.off[k] + (n + 1) // 2].view(f32 if k in ("temp", "topp") else i32)[:n]
+            out[k] = buf[self.off[k]:self.off[k] + (n + 1) // 2].view(f32 if k in ("temp", "topp", "minp") else i32)[:n]
         out["tables"] = out["tables"].reshape(self.nt, self.mb) if self.nt * self.mb else out["tables"]
         return out
 
@@ -159,7 +168,11 @@ class LLMEngine:
                  block_size: int = 16, num_blocks: int | None = None, gpu_memory_utilization: float = 0.85,
                  max_num_seqs: int = 256, max_num_batched_tokens: int = 8192, max_model_len: int | None = None,
                  use_cuda_graphs: bool = True, mixed_batches: bool = True, async_scheduling: bool = True,
-                 prefill_chunk: int = 0, enable_prefix_caching: bool = False):
+                 prefill_chunk: int = 0, enable_prefix_caching: bool = False, kv_cache_dtype: str = "auto",
+                 fork_samples: bool = False):
+        """kv_cache_dtype: "auto" keeps keys and values in the compute type, "fp8" in 8 bits with a scale for each page and head (Llama family):
+        half the memory and half the bytes a decode step reads. fork_samples: a request whose params.fork_of names a running one with the same
+        prompt shares that prompt's pages instead of running it again (the n answers of one API request)."""
         self.cfg, self.w, self.tp, self.tokenizer, self.info = cfg, weights, tp, tokenizer, info
         self.device = weights.embed.device
         self.dtype = weights.embed.dtype
@@ -176,17 +189,28 @@ class LLMEngine:
         if self.per_sequence and self.world > 1:
             raise ValueError(f"{cfg.name}: tensor parallelism is not available for this model family")
         kv_specs, state_specs = runner_cls.cache_specs(cfg, weights)
+        if kv_cache_dtype not in ("auto", "fp8"):
+            raise ValueError(f"kv_cache_dtype is \"auto\" or \"fp8\", not {kv_cache_dtype!r}")
+        kv8 = kv_cache_dtype == "fp8"
+        if kv8 and self.per_sequence:
+            raise ValueError(f"{cfg.name}: pages in 8 bits are available for the Llama family only")
+        if fork_samples and self.world > 1:
+            raise ValueError("fork_samples copies pages on one GPU only")
         self.slots = None
         if any(s is not None for s in state_specs):
             if enable_prefix_caching:
                 raise ValueError(f"{cfg.name}: prefix caching shares pages of keys and values, but this model also carries "
                                  "recurrent state from token to token")
+            if fork_samples:
+                raise ValueError(f"{cfg.name}: fork_samples shares pages of keys and values, but this model also carries recurrent state "
+                                 "from token to token")
             self.slots = SlotManager(max_num_seqs)
             self.states = StateCache(state_specs, max_num_seqs, self.dtype, self.device)
         else:
             self.states = None
         if num_blocks is None:
-            per_block = max(1, KVCache.bytes_per_block_specs(kv_specs, block_size, self.dtype))
+            per_block = max(1, KVCache8.bytes_per_block(len(kv_specs), block_size, kv_specs[0].kv_heads, kv_specs[0].dim) if kv8
+                            else KVCache.bytes_per_block_specs(kv_specs, block_size, self.dtype))
             if self.device.type == "cuda":
                 free, total = torch.cuda.mem_get_info(self.device)
                 budget = max(0, free - (1 - gpu_memory_utilization) * total - (2 << 30))
@@ -200,10 +224,13 @@ class LLMEngine:
                     num_blocks = int(t.item())
             else:
                 num_blocks = 256
-        self.kv = KVCache.from_specs(kv_specs, num_blocks, block_size, self.dtype, self.device)
+        if kv8:
+            self.kv = KVCache8(len(kv_specs), num_blocks, block_size, kv_specs[0].kv_heads, kv_specs[0].dim, self.device)
+        else:
+            self.kv = KVCache.from_specs(kv_specs, num_blocks, block_size, self.dtype, self.device)
         self.blocks = BlockManager(num_blocks, block_size, enable_prefix_caching)
         self.sched = Scheduler(self.blocks, max_num_seqs, max_num_batched_tokens, self.max_model_len,
-                               mixed=mixed_batches, prefill_chunk=prefill_chunk, slots=self.slots)
+                               mixed=mixed_batches, prefill_chunk=prefill_chunk, slots=self.slots, fork_samples=fork_samples)
         if self.per_sequence:
             self.runner = runner_cls(cfg, weights, self.kv, self.states, self.max_model_len)
         else:
@@ -293,7 +320,7 @@ class LLMEngine:
                   want=None) -> "PackedStep":
         """Lay one step's metadata out in a pinned host buffer (see StepLayout). ids/pos/slots cover all T
         rows (decode rows first); ctx/tables the nd decode rows; cu the packed prompts (relative to row nd);
-        sampling = (temperature, top_k, top_p, seeds) per sampled row or None. sampled_prompts: how many of the
+        sampling = (temperature, top_k, top_p, seeds[, min_p]) per sampled row or None. sampled_prompts: how many of the
         prompts (the first ones) end in this step; prefix = (pslots, pdst, csrc, ecu, max_ext) when prompt rows
         continue prompts whose earlier tokens are in the cache.
         For a runner with per_sequence = True, ctx / tables / sslots (state slots) cover the prompts too and starts[i]
@@ -312,8 +339,11 @@ class LLMEngine:
         ns = npf if sampled_prompts is None else sampled_prompts
         mb = max((len(t) for t in tables), default=0)
         mb = (mb + 7) & ~7
+        # min-p, or a vocabulary that `sample` does not hold: the step brings its random numbers
+        min_p = sampling[4] if sampling is not None and len(sampling) > 4 else ()
+        given = sampling is not None and (any(min_p) or (self.device.type == "cuda" and self.cfg.vocab_size > S.SAMPLE_MAX))
         lay = StepLayout(T, nd, npf, mb, ns, len(prefix[0]) if prefix is not None else 0, full, nsg,
-                         None if want is None else len(want))
+                         None if want is None else len(want), given)
         slot = self._host_buffer("step", lay.words)
         v = lay.views(slot[0].numpy(), np)
         v["ids"][:] = ids
@@ -346,7 +376,10 @@ class LLMEngine:
         if prefix is not None:
             v["pslots"][:], v["pdst"][:], v["csrc"][:], v["ecu"][:] = prefix[:4]
         if sampling is not None:
-            v["temp"][:], v["topk"][:], v["topp"][:], v["seeds"][:] = sampling
+            v["temp"][:], v["topk"][:], v["topp"][:], v["seeds"][:] = sampling[:4]
+        if given:
+            v["minp"][:] = min_p if len(min_p) else 0.0
+            v["unif"][:] = uniforms(v["seeds"])
         return PackedStep(lay, slot, int(max_seqlen), int(prefix[4]) if prefix is not None else 0, seg_at)
 
     def _pack_batch(self, batch: Batch, want=None, given: dict | None = None) -> "PackedStep":
@@ -407,7 +440,8 @@ class LLMEngine:
                     [r.params.top_p for r in reqs],
                     # random stream keyed by (request seed, index of the token being generated): same seed =>
                     # same text, whatever else the engine is doing
-                    [(r.seed * 1000003 + len(r.output_ids) + r.pending) & 0x7FFFFFFFFFFFFFFF for r in reqs])
+                    [(r.seed * 1000003 + len(r.output_ids) + r.pending) & 0x7FFFFFFFFFFFFFFF for r in reqs],
+                    [r.params.min_p for r in reqs])
         return self.pack_step(nd, ids, pos, slots, ctx, tables, cu, max_seqlen, sampling, src,
                               sampled_prompts=batch.num_sampled - nd, prefix=prefix, sslots=sslots, starts=starts,
                               want=want)
@@ -448,15 +482,15 @@ class LLMEngine:
                 lay = step.layout
                 msg = np.empty(12 + lay.words, dtype=np.int64)
                 msg[:12] = [0, lay.T, lay.nd, lay.npf, lay.mb, step.max_seqlen, lay.words, int(step.want_lp), lay.ns,
-                            lay.P, step.max_ext, 0]
+                            lay.P, step.max_ext, int(lay.given)]
                 msg[12:] = step.slot[0][:lay.words].numpy()
                 ring.write(msg)
                 return step
             raw = ring.read().view(np.int64)
-            kind, T, nd, npf, mb, max_seqlen, words, want_lp, ns, P, max_ext = (int(x) for x in raw[:11])
+            kind, T, nd, npf, mb, max_seqlen, words, want_lp, ns, P, max_ext, given = (int(x) for x in raw[:12])
             if kind < 0:
                 return None
-            lay = StepLayout(T, nd, npf, mb, ns, P)
+            lay = StepLayout(T, nd, npf, mb, ns, P, given=bool(given))
             slot = self._host_buffer("step", words)
             slot[0][:words].numpy()[:] = raw[12:12 + words]
             step = PackedStep(lay, slot, max_seqlen, max_ext)
@@ -469,15 +503,15 @@ class LLMEngine:
                 return None
             lay = step.layout
             dist.broadcast(torch.tensor([0, lay.T, lay.nd, lay.npf, lay.mb, step.max_seqlen, lay.words,
-                                         int(step.want_lp), lay.ns, lay.P, step.max_ext, 0], dtype=torch.int64), 0)
+                                         int(step.want_lp), lay.ns, lay.P, step.max_ext, int(lay.given)], dtype=torch.int64), 0)
             dist.broadcast(step.slot[0][:lay.words], 0)
             return step
         hdr = torch.zeros(12, dtype=torch.int64)
         dist.broadcast(hdr, 0)
-        kind, T, nd, npf, mb, max_seqlen, words, want_lp, ns, P, max_ext = (int(x) for x in hdr[:11])
+        kind, T, nd, npf, mb, max_seqlen, words, want_lp, ns, P, max_ext, given = (int(x) for x in hdr[:12])
         if kind < 0:
             return None
-        lay = StepLayout(T, nd, npf, mb, ns, P)
+        lay = StepLayout(T, nd, npf, mb, ns, P, given=bool(given))
         slot = self._host_buffer("step", words)
         dist.broadcast(slot[0][:words], 0)
         step = PackedStep(lay, slot, max_seqlen, max_ext)
@@ -514,6 +548,9 @@ class LLMEngine:
             return self._tok_dev[:0], None
         if B > self._tok_dev.numel():
             raise RuntimeError(f"{B} sampled rows exceed the sample buffer ({self._tok_dev.numel()})")
+        if step.layout.given:
+            return S.sample_given(logits, v["unif"], v["temp"], v["topk"], v["topp"], v["minp"], want_logprob=want_lp,
+                                  out=self._tok_dev[:B])
         toks, lps = S.sample(logits, v["temp"], v["topk"], v["topp"], v["seeds"], step=0, want_logprob=want_lp,
                              out=self._tok_dev[:B])
         return toks, lps
@@ -527,7 +564,7 @@ class LLMEngine:
         dev, mbs = self.device, self.max_blocks_per_seq
         g = self.graphs.get(bucket)
         if g is None:
-            glay = StepLayout(bucket, bucket, 0, mbs, full=self.per_sequence)
+            glay = StepLayout(bucket, bucket, 0, mbs, full=self.per_sequence, given=True)
             buf = torch.zeros(glay.words, dtype=torch.int64, device=dev)
             st = glay.views(buf, torch)
             st["slots"].fill_(-1)
@@ -556,7 +593,7 @@ class LLMEngine:
         slot = self._host_buffer(("graph", bucket), glay.words)
         src = lay.views(step.slot[0].numpy(), np)
         dst = glay.views(slot[0].numpy(), np)
-        for k in ("ids", "pos", "seeds", "topk", "temp", "topp"):
+        for k in ("ids", "pos", "seeds", "topk", "temp", "topp", *(("unif", "minp") if lay.given else ())):
             dst[k][:B] = src[k]
         dst["src"][:B] = src["src"]
         dst["src"][B:] = -1
@@ -572,7 +609,7 @@ class LLMEngine:
         dst["tables"][:B, :w] = src["tables"][:, :w]
         self._to_device(slot, glay.tables + (B * mbs + 1) // 2, buf)
         graph.replay()
-        return out[:B], {k: t[:B] for k, t in st.items() if k in ("temp", "topk", "topp", "seeds")}
+        return out[:B], {k: t[:B] for k, t in st.items() if k in ("temp", "topk", "topp", "minp", "seeds", "unif")}
 
     def step(self) -> list[StepOutput]:
         """Driver: schedule and launch one model step on all ranks, then hand back the results of the step
@@ -591,6 +628,8 @@ class LLMEngine:
 
     def _launch(self, batch: Batch) -> dict:
         reqs = batch.requests[:batch.num_sampled]          # rows that produce a token in this step
+        if batch.copies:                                   # pages that forked sequences go on from (stream order: before the step writes any)
+            self.kv.copy_pages(*(list(p) for p in zip(*batch.copies)))
         packed = self._pack_batch(batch)
         want_lp = any(r.params.logprobs is not None for r in reqs)
         packed.want_lp = want_lp

@@ -1,6 +1,6 @@
 """Paged KV cache: fixed-size blocks + per-sequence block tables (vLLM's
 PagedAttention memory model, restated). Tensors: k_cache, v_cache = [L][num_blocks, block_size,
-KV_heads_local, head_dim] in the compute dtype; the block manager is pure host-side bookkeeping.
+KV_heads_local, head_dim] in the compute dtype, or in 8 bits (KVCache8); the block manager is pure host-side bookkeeping.
 Layers with recurrent state keep it in a StateCache: one slot per sequence, handed out by a SlotManager."""
 from __future__ import annotations
 
@@ -9,11 +9,13 @@ from dataclasses import dataclass
 
 import torch
 
+from ..ops.pages import copy_pages
+
 
 class BlockManager:
     """Free list + (optional) prefix cache over fixed-size KV blocks.
 
-    Without prefix caching a block belongs to exactly one sequence. With `enable_prefix_caching` a FULL block
+    Without prefix caching a block belongs to exactly one sequence, or to several that were forked from one another. With `enable_prefix_caching` a FULL block
     whose content is determined by the token prefix it ends (hash chain over block_size-token groups, as in vLLM's
     automatic prefix caching, SP:vllm/v1/core/kv_cache_utils.py) is registered under that hash when its sequence
     has written it; a later prompt that starts with the same tokens takes a reference on the block instead of
@@ -59,9 +61,10 @@ class BlockManager:
     def release(self, blocks: list[int]) -> None:
         if not self.prefix_caching:
             for b in reversed(blocks):             # most recently freed first (warm in L2), blocks[0] at the front
-                self.ref[b] = 0
-                self.free[b] = None
-                self.free.move_to_end(b, last=False)
+                self.ref[b] -= 1
+                if self.ref[b] == 0:
+                    self.free[b] = None
+                    self.free.move_to_end(b, last=False)
             blocks.clear()
             return
         for b in reversed(blocks):                 # oldest-freed-first reuse: new entries go to the BACK, tail first
@@ -69,6 +72,21 @@ class BlockManager:
             if self.ref[b] == 0:
                 self.free[b] = None
         blocks.clear()
+
+    def fork(self, blocks: list[int], num_tokens: int) -> tuple[list[int], list[tuple[int, int]]] | None:
+        """Blocks of a new sequence that goes on from the first num_tokens tokens of the one that holds `blocks`: the full ones are shared (a
+        reference each), of one that is partly filled it gets a copy. Returns (blocks, copies to make as (from, to)), or None (nothing changed) if
+        out of blocks. The tokens from num_tokens on are the new sequence's own: it never writes a shared block."""
+        full, rest = divmod(num_tokens, self.block_size)
+        if rest and not self.free:
+            return None
+        out = list(blocks[:full])
+        for b in out:
+            self.ref[b] += 1
+        if not rest:
+            return out, []
+        out.append(self._take())
+        return out, [(blocks[full], out[-1])]
 
     # ---- prefix cache -----------------------------------------------------------------------------
     def _chain(self, tokens: list[int], n_blocks: int):
@@ -219,6 +237,33 @@ class KVCache:
         es = torch.empty(0, dtype=dtype).element_size()
         return sum(block_size * s.kv_heads * (s.dim + s.vdim) * es for s in specs if s is not None and s.source is None)
 
+    def copy_pages(self, src: list[int], dst: list[int]) -> None:
+        """Pages src[i] -> dst[i] of every layer."""
+        mine = {id(t): t for t in (*self.k, *self.v) if t is not None and t.numel()}
+        copy_pages(list(mine.values()), src, dst)
+
     @staticmethod
     def bytes_per_block(num_layers, block_size, kv_heads, head_dim, dtype) -> int:
         return 2 * num_layers * block_size * kv_heads * head_dim * torch.empty(0, dtype=dtype).element_size()
+
+
+class KVCache8:
+    """Pages in 8 bits (ops/kv8.py): per layer k[l], v[l] [num_blocks, KV, block_size, head_dim] e4m3 and k_scale[l], v_scale[l] [num_blocks, KV]
+    fp32, views of one tensor for all layers. Half the bytes of KVCache, so twice the tokens in the same memory."""
+
+    def __init__(self, num_layers: int, num_blocks: int, block_size: int, kv_heads: int, head_dim: int, device):
+        if block_size < 8 or block_size % 8:
+            raise ValueError(f"pages in 8 bits hold a multiple of 8 tokens, not {block_size}")
+        shape = (num_layers, num_blocks, kv_heads, block_size, head_dim)
+        self._all = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+        self._all += [torch.full(shape[:3], 2.0 ** -120, dtype=torch.float32, device=device) for _ in range(2)]
+        self.k, self.v, self.k_scale, self.v_scale = (list(t.unbind(0)) for t in self._all)
+        self.num_blocks, self.block_size = num_blocks, block_size
+
+    def copy_pages(self, src: list[int], dst: list[int]) -> None:
+        """Pages src[i] -> dst[i] of every layer, with their scales."""
+        copy_pages(self._all, src, dst, page_dim=1)
+
+    @staticmethod
+    def bytes_per_block(num_layers, block_size, kv_heads, head_dim) -> int:
+        return 2 * num_layers * kv_heads * (block_size * head_dim + 4)

@@ -24,9 +24,10 @@ import torch
 from ..models.config import LlamaConfig
 from ..ops import attention as A
 from ..ops import elementwise as E
+from ..ops import kv8 as K8
 from ..ops import serving as S
 from ..ops.gemm import gemm, gemm_skinny, gemm_skinny_acc, gemm_swiglu
-from .kv_cache import KVCache, KVSpec
+from .kv_cache import KVCache, KVCache8, KVSpec
 
 
 _FUSE_ACC = os.environ.get("DLTI_DECODE_FUSE_ACC", "1") == "1"    # A/B switch: consume the fp32 accumulators directly
@@ -343,8 +344,9 @@ class ModelRunner:
         """(key/value page specs, recurrent-state specs), one entry per layer."""
         return [KVSpec(weights.KV, cfg.head_dim, cfg.head_dim)] * cfg.num_hidden_layers, [None] * cfg.num_hidden_layers
 
-    def __init__(self, cfg: LlamaConfig, weights: TPWeights, kv: KVCache, tp: TPContext):
+    def __init__(self, cfg: LlamaConfig, weights: TPWeights, kv: KVCache | KVCache8, tp: TPContext):
         self.cfg, self.w, self.kv, self.tp = cfg, weights, kv, tp
+        self.kv8 = isinstance(kv, KVCache8)
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
         self.cos, self.sin = E.rope_tables(cfg.max_position_embeddings, cfg.head_dim, cfg.rope_theta,
                                            weights.embed.device)
@@ -354,6 +356,41 @@ class ModelRunner:
             # serving weights are static: the decode GEMMs may fetch weight tiles while the previous kernel drains
             from ..ops import _lib
             _lib.gpu_lib().dlti_set_pdl(2)
+
+    # ---- a layer's cache: pages in the compute type, or in 8 bits -------------------------------------------
+    def _pages8(self, li: int):
+        kv = self.kv
+        return kv.k[li], kv.v[li], kv.k_scale[li], kv.v_scale[li], self.w.H, self.w.KV, self.cfg.head_dim
+
+    def _cache_rows(self, li: int, qkv, pos, slots) -> None:
+        """Rotate q and k of the rows in place; rotated k and v go to the cache."""
+        if self.kv8:
+            K8.rope_cache8_(qkv, pos, self.cos, self.sin, slots, *self._pages8(li))
+        else:
+            S.rope_cache_(qkv, pos, self.cos, self.sin, slots, self.kv.k[li], self.kv.v[li], self.w.H, self.w.KV, self.cfg.head_dim)
+
+    def _cache_acc(self, li: int, acc, dtype, pos, slots):
+        """The same from the decode GEMM's accumulator; returns the 16-bit rows."""
+        if self.kv8:
+            return K8.acc_rope_cache8(acc, dtype, pos, self.cos, self.sin, slots, *self._pages8(li))
+        return S.acc_rope_cache(acc, dtype, pos, self.cos, self.sin, slots, self.kv.k[li], self.kv.v[li], self.w.H, self.w.KV, self.cfg.head_dim)
+
+    def _decode(self, li: int, q, tables, ctx, max_ctx, out=None):
+        """Attention of single tokens over the cache."""
+        if self.kv8:
+            k, v, ks, vs, *heads = self._pages8(li)
+            return K8.paged_decode8(q, k, v, ks, vs, tables, ctx, *heads, self.scale, out=out, max_ctx=max_ctx)
+        return S.paged_decode(q, self.kv.k[li], self.kv.v[li], tables, ctx, self.w.H, self.w.KV, self.cfg.head_dim, self.scale, out=out,
+                              max_ctx=max_ctx)
+
+    def _cached_rows(self, li: int, ext, rows, slots) -> None:
+        """Keys and values of cached tokens to the rows `rows` of ext."""
+        H, KV, hd = self.w.H, self.w.KV, self.cfg.head_dim
+        if self.kv8:
+            K8.gather_rows8_(ext, rows, slots, *self._pages8(li))
+        else:
+            ext[rows, H * hd:(H + KV) * hd] = self.kv.k[li].view(-1, KV * hd)[slots]
+            ext[rows, (H + KV) * hd:] = self.kv.v[li].view(-1, KV * hd)[slots]
 
     @torch.no_grad()
     def forward(self, input_ids, positions, slots, *, num_decode: int = 0, block_tables=None, ctx_lens=None,
@@ -411,38 +448,32 @@ class ModelRunner:
                 if acc_path:
                     acc = gemm_skinny_acc(x_in, lw["w_qkv"])
                     gemm_skinny_acc(t, ad["B_qkv"])
-                    qkv = S.acc_rope_cache(acc, x_in.dtype, positions, self.cos, self.sin, slots, self.kv.k[li],
-                                           self.kv.v[li], H, KV, hd)
+                    qkv = self._cache_acc(li, acc, x_in.dtype, positions, slots)
                 else:
                     qkv = gemm(x_in, lw["w_qkv"], a2=t, b2=ad["B_qkv"])
-                    S.rope_cache_(qkv, positions, self.cos, self.sin, slots, self.kv.k[li], self.kv.v[li], H, KV, hd)
+                    self._cache_rows(li, qkv, positions, slots)
             elif acc_path:
-                qkv = S.acc_rope_cache(gemm_skinny_acc(xn, lw["w_qkv"]), xn.dtype, positions, self.cos, self.sin,
-                                       slots, self.kv.k[li], self.kv.v[li], H, KV, hd)
+                qkv = self._cache_acc(li, gemm_skinny_acc(xn, lw["w_qkv"]), xn.dtype, positions, slots)
             else:
                 qkv = colpar(xn, lw["w_qkv"])
-                S.rope_cache_(qkv, positions, self.cos, self.sin, slots, self.kv.k[li], self.kv.v[li], H, KV, hd)
+                self._cache_rows(li, qkv, positions, slots)
             if prefix is not None:
                 attn = torch.empty((T, H * hd), dtype=qkv.dtype, device=qkv.device)
                 if nd:
-                    S.paged_decode(qkv[:nd], self.kv.k[li], self.kv.v[li], block_tables, ctx_lens, H, KV, hd,
-                                   self.scale, out=attn[:nd], max_ctx=max_ctx)
+                    self._decode(li, qkv[:nd], block_tables, ctx_lens, max_ctx, out=attn[:nd])
                 pslots, pdst, csrc, ecu, max_ext = prefix
                 ext = torch.zeros((int(pdst.numel() + csrc.numel()), qkv.shape[1]), dtype=qkv.dtype, device=qkv.device)
                 ext[csrc] = qkv[nd:]
-                ext[pdst, H * hd:(H + KV) * hd] = self.kv.k[li].view(-1, KV * hd)[pslots]
-                ext[pdst, (H + KV) * hd:] = self.kv.v[li].view(-1, KV * hd)[pslots]
+                self._cached_rows(li, ext, pdst, pslots)
                 out_ext, _ = A.attention_fwd(ext, ecu, max_ext, H, KV, hd, self.scale, want_lse=False)
                 attn[nd:] = out_ext[csrc]
             elif nd == 0:
                 attn, _ = A.attention_fwd(qkv, cu_seqlens, max_seqlen, H, KV, hd, self.scale, want_lse=False)
             elif nd == T:
-                attn = S.paged_decode(qkv, self.kv.k[li], self.kv.v[li], block_tables, ctx_lens, H, KV, hd,
-                                      self.scale, max_ctx=max_ctx)
+                attn = self._decode(li, qkv, block_tables, ctx_lens, max_ctx)
             else:
                 attn = torch.empty((T, H * hd), dtype=qkv.dtype, device=qkv.device)
-                S.paged_decode(qkv[:nd], self.kv.k[li], self.kv.v[li], block_tables, ctx_lens, H, KV, hd,
-                               self.scale, out=attn[:nd], max_ctx=max_ctx)
+                self._decode(li, qkv[:nd], block_tables, ctx_lens, max_ctx, out=attn[:nd])
                 A.attention_fwd(qkv[nd:], cu_seqlens, max_seqlen, H, KV, hd, self.scale, want_lse=False,
                                 out=attn[nd:])
             if ad is not None and ad["A_o"] is not None:

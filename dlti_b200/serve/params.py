@@ -12,6 +12,7 @@ class SamplingParams:
     temperature: float = 1.0
     top_p: float = 1.0
     top_k: int = 0              # 0 / -1 = off
+    min_p: float = 0.0          # tokens less likely than min_p times the likeliest are not drawn (0 = off)
     n: int = 1
     seed: int | None = None
     stop: list[str] = field(default_factory=list)
@@ -22,6 +23,7 @@ class SamplingParams:
     echo: bool = False
     skip_special_tokens: bool = True
     detokenize: bool = True     # False (vLLM's field of the same name): return token ids only, produce no text
+    fork_of: str | None = None  # request with the same prompt whose pages this one may share (LLMEngine(fork_samples=True))
 
     def __post_init__(self):
         if isinstance(self.stop, str):
@@ -31,7 +33,8 @@ class SamplingParams:
             self.top_k = 0
         if self.max_tokens is None:
             self.max_tokens = 16
-        if self.temperature < 0 or not (0 < self.top_p <= 1.0) or self.max_tokens < 1 or self.n < 1:
+        if (self.temperature < 0 or not (0 < self.top_p <= 1.0) or not (0 <= self.min_p <= 1.0) or self.max_tokens < 1
+                or self.n < 1):
             raise ValueError("invalid sampling parameters")
 
 

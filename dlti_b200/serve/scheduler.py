@@ -9,7 +9,7 @@ is preempted (blocks freed, re-queued at the front; its tokens are recomputed on
 from __future__ import annotations
 
 from collections import deque
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 from .kv_cache import BlockManager, SlotManager
 from .params import Request
@@ -21,6 +21,7 @@ class Batch:
     requests: list[Request]      # decode rows first, then prompts that complete in this step, then partial prompts
     num_decode: int = 0
     num_sampled: int = -1        # requests[:num_sampled] get a token from this step (-1 = all)
+    copies: list = field(default_factory=list)   # pages (from, to) to copy before the step
 
     def __post_init__(self):
         if self.num_sampled < 0:
@@ -30,7 +31,7 @@ class Batch:
 class Scheduler:
     def __init__(self, blocks: BlockManager, max_num_seqs: int = 256, max_num_batched_tokens: int = 8192,
                  max_model_len: int = 4096, mixed: bool = True, prefill_chunk: int = 0,
-                 slots: SlotManager | None = None):
+                 slots: SlotManager | None = None, fork_samples: bool = False):
         self.blocks = blocks
         self.slots = slots           # recurrent-state slots, for models that carry state from token to token
         self.mixed = mixed           # False = prefill-first steps (no decode rows in a prefill pass)
@@ -43,6 +44,9 @@ class Scheduler:
         self.waiting: deque[Request] = deque()
         self.running: list[Request] = []
         self.num_preemptions = 0
+        # a request that names another one with the same prompt (params.fork_of) starts from that one's pages instead of running the prompt again
+        self.fork_samples = fork_samples
+        self.num_forks = 0
 
     def add(self, req: Request) -> None:
         if len(req.prompt_ids) + 1 > self.max_model_len:
@@ -84,6 +88,49 @@ class Scheduler:
         r.blocks.extend(self.blocks.match_prefix(r.prompt_ids + r.output_ids))
         return len(r.blocks) * self.blocks.block_size
 
+    def _origin(self, r: Request) -> Request | None:
+        """The running request whose prompt pages the waiting request r may share."""
+        if not self.fork_samples or r.params.fork_of is None or r.output_ids or r.pending or r.blocks:
+            return None
+        for p in self.running:
+            if p.request_id == r.params.fork_of and p.prompt_ids == r.prompt_ids:
+                return p
+        return None
+
+    def _waits_for_origin(self, r: Request, admitted: list[Request]) -> bool:
+        """Whether r is a fork of a request whose prompt is on its way into the cache: of one admitted in this step, or of a running one."""
+        if not self.fork_samples or r.params.fork_of is None or r.output_ids:
+            return False
+        return self._origin(r) is not None or any(p.request_id == r.params.fork_of and p.prompt_ids == r.prompt_ids for p in admitted)
+
+    def _admit_forks(self, decode: list[Request], room: int) -> list[tuple[int, int]]:
+        """Waiting requests whose origin has its whole prompt in the cache join the decode rows (at most `room`): they share the pages of all prompt
+        tokens but the last, which is their first row. Ones whose origin is still at its prompt wait for it; the others stay as they were. Returns
+        the pages to copy."""
+        copies = []
+        if not self.fork_samples:
+            return copies
+        for r in [q for q in self.waiting if q.params.fork_of is not None]:
+            if room <= 0 or len(self.running) >= self.max_num_seqs:
+                break
+            p = self._origin(r)
+            if p is None or not p.prefill_done or p.sched_tokens <= len(p.prompt_ids):
+                continue
+            n = len(r.prompt_ids)
+            if not self.blocks.can_allocate(n + 1, (n - 1) // self.blocks.block_size):
+                break
+            blocks, more = self.blocks.fork(p.blocks, n - 1)
+            r.blocks.extend(blocks)
+            self.blocks.ensure(r.blocks, n + 1)
+            copies += more
+            self.waiting.remove(r)
+            r.status, r.num_computed, r.chunk, r.prefill_done = "running", n, 0, True
+            self.running.append(r)
+            decode.append(r)
+            self.num_forks += 1
+            room -= 1
+        return copies
+
     def _at_limit(self, r: Request) -> bool:
         return (len(r.output_ids) + r.pending >= r.params.max_tokens) or r.sched_tokens >= self.max_model_len
 
@@ -116,13 +163,18 @@ class Scheduler:
             self.num_preemptions += 1
             preempted = True
         decode = [r for r in self.running if not self._at_limit(r)]
+        copies = [] if preempted else self._admit_forks(decode, self.max_num_batched_tokens - len(decode))
         # ---- prefill rows: admit waiting prompts FCFS (not in a step that had to preempt) ----
         admitted: list[Request] = []
+        held: list[Request] = []                  # forks whose origin's prompt is part of this step: they come with the next one
         budget = self.max_num_batched_tokens - len(decode)
         while self.waiting and not preempted and len(self.running) + len(admitted) < self.max_num_seqs:
             r = self.waiting[0]
             if r.pending:                         # preempted with a sampled token still unread: next step
                 break
+            if self._waits_for_origin(r, admitted):
+                held.append(self.waiting.popleft())
+                continue
             n = r.num_tokens                      # prompt (+ already generated tokens if it was preempted)
             have = self._take_cached_prefix(r)    # tokens already in the cache (prefix caching), else 0
             if (n - have > budget and (admitted or decode)) or not self._acquire(r, n + 1):
@@ -135,15 +187,16 @@ class Scheduler:
             budget -= n - have
             if budget <= 0:
                 break
+        self.waiting.extendleft(reversed(held))
         if admitted and decode and not self.mixed:
             # prefill-first policy (vLLM v0 style): a step is either all prompts or all decode rows
             self.running.extend(admitted)
-            return Batch("prefill", admitted, 0)
+            return Batch("prefill", admitted, 0, copies=copies)
         self.running.extend(admitted)
         if not decode and not admitted:
             return None
         kind = "mixed" if decode and admitted else ("prefill" if admitted else "decode")
-        return Batch(kind, decode + admitted, len(decode))
+        return Batch(kind, decode + admitted, len(decode), copies=copies)
 
     def _schedule_chunked(self) -> Batch | None:
         """schedule() with chunked prefill: prompts enter the cache `prefill_chunk` tokens at a time (and never
@@ -162,6 +215,7 @@ class Scheduler:
             self._unschedule(victim)
             preempted = True
         decode = [r for r in self.running if r.prefill_done and not self._at_limit(r)]
+        copies = [] if preempted else self._admit_forks(decode, self.max_num_batched_tokens - len(decode))
         budget = self.max_num_batched_tokens - (len(decode) if self.mixed else 0)
         complete, partial = [], []
 
@@ -184,11 +238,15 @@ class Scheduler:
                 break
         stalled = any(not r.prefill_done and r not in complete and r not in partial for r in self.running)
         admitted = []
+        held = []
         while (self.waiting and not preempted and not stalled and budget > 0
                and len(self.running) + len(admitted) < self.max_num_seqs):
             r = self.waiting[0]
             if r.pending:
                 break
+            if self._waits_for_origin(r, admitted):
+                held.append(self.waiting.popleft())
+                continue
             r.num_computed, r.prefill_done = self._take_cached_prefix(r), False
             if not take(r):
                 self.release(r)
@@ -197,6 +255,7 @@ class Scheduler:
             self.waiting.popleft()
             r.status = "running"
             admitted.append(r)
+        self.waiting.extendleft(reversed(held))
         self.running.extend(admitted)
         prompts = complete + partial
         if prompts and decode and not self.mixed:
@@ -207,7 +266,7 @@ class Scheduler:
                 return self._schedule_chunked()
             return None
         kind = "mixed" if decode and prompts else ("prefill" if prompts else "decode")
-        return Batch(kind, decode + prompts, len(decode), len(decode) + len(complete))
+        return Batch(kind, decode + prompts, len(decode), len(decode) + len(complete), copies=copies)
 
     def _unschedule(self, victim: Request) -> None:
         self.release(victim)

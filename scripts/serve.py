@@ -69,7 +69,7 @@ def make_engine(a, info, cfg, w, tp, tok):
                     max_num_batched_tokens=a.max_num_batched_tokens, max_model_len=a.max_model_len,
                     use_cuda_graphs=not a.enforce_eager, mixed_batches=not a.no_mixed_batches,
                     async_scheduling=not a.no_async_scheduling, prefill_chunk=a.prefill_chunk,
-                    enable_prefix_caching=a.enable_prefix_caching)
+                    enable_prefix_caching=a.enable_prefix_caching, kv_cache_dtype=a.kv_cache_dtype, fork_samples=a.fork_samples)
     if info.rank == 0 and not a.no_warmup:
         eng.warmup()                      # workers follow from worker_loop()
     return eng
@@ -101,6 +101,10 @@ def add_args(ap):
                     help="> 0: chunked prefill, at most this many tokens of one prompt per step (experimental)")
     ap.add_argument("--enable_prefix_caching", action="store_true",
                     help="share the KV blocks of a common prompt prefix between requests (experimental)")
+    ap.add_argument("--kv_cache_dtype", default="auto", choices=["auto", "fp8"],
+                    help="fp8: keys and values in 8 bits with a scale for each page and head (Llama family)")
+    ap.add_argument("--fork_samples", action="store_true",
+                    help="the n answers of a request share the pages of its prompt, which runs once")
     ap.add_argument("--no_warmup", action="store_true", help="capture the decode CUDA graphs lazily")
     ap.add_argument("--no_async_scheduling", action="store_true",
                     help="read each step's tokens on the host before launching the next step")
