@@ -259,10 +259,12 @@ int rows8_t(const Rows8& p, cudaStream_t st) {
 // Attention of single tokens. A CTA takes one split of one sequence's context for up to 8 query heads of one key/value head; its warps take
 // tiles of 16 tokens in turn and never wait for one another before the end.
 //
-// Both products are m16n8k16 in fp16 with fp32 sums: e4m3 numbers are fp16 numbers. Neither operand passes through shared memory. The order
-// of the contraction is free as long as both operands agree, so a lane takes 16 consecutive bytes of a key (dimensions 64 i + 16 t ...) as its
-// share of four k-steps, and 16 consecutive bytes of four values (tokens 2t, 2t+1, 2t+8, 2t+9, dimensions 16 g ...) as the columns g of 16
-// n-tiles: bytes of neighbouring tokens are paired by a permute.
+// Each warp has a ring of tiles of its own in shared memory, filled by cp.async (16 bytes a lane; the 16-byte pieces of a row change places with
+// the row, so that neither the writes nor the two kinds of reads meet in a bank).
+// Both products are m16n8k16 in fp16 with fp32 sums: e4m3 numbers are fp16 numbers. The order of the contraction is free as long as both
+// operands agree, so a lane takes 32 consecutive numbers of a key (dimensions 32 t ...) as its share of the eight k-steps, and 16 consecutive
+// numbers of four values (tokens 2t, 2t+1, 2t+8, 2t+9, dimensions 16 g ...) as the columns g of 16 n-tiles: bytes of neighbouring tokens are
+// paired by a permute.
 //   queries: scaled by a power of two per head so that their 16 bits are fp16 numbers exactly (down to 2^-39 of the head's largest);
 //   weights p s_v: p <= 1 times the page's value scale over the largest seen so far, as fp16 hi + lo, rows g and g + 8 of the same product:
 //   22 bits, absolutely 2^-40 of the largest.
@@ -279,12 +281,33 @@ __device__ __forceinline__ float ex2f(float x) {
 __device__ __forceinline__ uint32_t word(const int4& v, int i) { return (uint32_t)(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w); }
 
 constexpr int NW = 4;            // warps of a CTA
+constexpr int RING = 3;          // tiles of a warp in flight or in use
 constexpr float P_UNIT = 32768.f;
 
-struct Tile {
-  int4 k[2][2], v[2][2];         // [half of 8 tokens][64 dimensions], [half][token of a pair]
-  float ks[2], vs[2];
+struct __align__(128) Stage {
+  uint8_t k[16][128], v[16][128];
 };
+constexpr int PITCH = HD + 4;
+union AttendSmem {
+  Stage ring[NW][RING];
+  float o[NW][8][PITCH];         // joining the warps
+};
+
+// both halves of a word as fp16 pairs
+__device__ __forceinline__ void half4_of_e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ int4 lds128(uint32_t a) {
+  int4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int n) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, int n) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
 
 struct Attend8 {
   const void* q;
@@ -292,7 +315,7 @@ struct Attend8 {
   const uint8_t *k8, *v8;
   const float *ks, *vs;
   const int *tables, *ctx;
-  int max_blocks, bs, G, KV, splits;
+  int max_blocks, bs, shift, G, KV, splits;      // shift: bs = 1 << shift, or -1
   float scale_log2;
   float *part_o, *part_ml;       // [batch, heads, splits, 128], [..., 2]
   void* out;
@@ -300,7 +323,11 @@ struct Attend8 {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
+__global__ void __launch_bounds__(32 * NW, 4) attend8_kernel(const Attend8 p) {
+  extern __shared__ __align__(128) unsigned char raw[];
+  AttendSmem& sm = *reinterpret_cast<AttendSmem*>(raw);
+  __shared__ float s_m[NW][8], s_l[NW][8];
+  __shared__ __align__(16) float s_scale[NW][RING][4];      // of a tile's halves: keys, values
   griddep_pass(gridDim.z);
   const int split = blockIdx.x, b = blockIdx.z;
   const int groups = (p.G + 7) / 8;
@@ -313,31 +340,64 @@ __global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
   const int end = min(tiles, (split + 1) * per);
   int tile = split * per + warp;
 
+  // ---- the ring
+  const int* table = p.tables + (long long)b * p.max_blocks;
+  const uint32_t ring = smem_u32(&sm.ring[warp][0]), scales = smem_u32(&s_scale[warp][0][0]);
+  const int r8 = lane >> 3, c16 = (lane & 7) * 16;          // a lane copies bytes c16 .. of rows r8, r8 + 4, ... of a tile
+  auto page_at = [&](int tb) { return p.shift >= 0 ? tb >> p.shift : (int)((uint32_t)tb / (uint32_t)p.bs); };
+  // pages of a tile's halves; a half that begins at or after the end has none
+  auto pages = [&](int at, int (&pg)[2]) {
+    const int tb = at * 16;
+    pg[0] = at < end ? table[page_at(tb)] : -1;
+    pg[1] = at < end && tb + 8 < ctx ? table[page_at(tb + 8)] : -1;
+  };
+  auto fill = [&](int at, const int (&pg)[2], int slot) {
+    if (at < end) {
+      const uint32_t dst = ring + slot * (uint32_t)sizeof(Stage);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool ok = pg[h] >= 0;
+        const long long sc = ok ? (long long)pg[h] * p.KV + kvh : 0;
+        const int tb = at * 16 + 8 * h, off = tb - page_at(tb) * p.bs;
+        const long long base = ok ? (sc * p.bs + off) * HD + r8 * HD + c16 : 0;
+        const int n = ok ? 16 : 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = r8 + 4 * i;
+          const uint32_t d = dst + (8 * h + r) * 128 + (c16 ^ (r << 4));
+          cp16(d, p.k8 + base + i * 4 * HD, n);
+          cp16(d + 16 * 128, p.v8 + base + i * 4 * HD, n);
+        }
+        if ((lane >> 1) == h) {                             // lanes 2 h, 2 h + 1: this half's scales
+          const bool v = lane & 1;
+          cp4(scales + (slot * 4 + 2 * v + h) * 4, (v ? p.vs : p.ks) + sc, ok ? 4 : 0);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int pg[2];
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) {
+    pages(tile + i * NW, pg);
+    fill(tile + i * NW, pg, i);
+  }
+  pages(tile + (RING - 1) * NW, pg);
+
+  // ---- the queries
   uint32_t aq[8][2];
   float fq = 0.f;
   {
-    float f[2][16], top = 0.f;
-    if (g < nh) {
-      const T* qp = reinterpret_cast<const T*>(p.q) + b * p.q_ld + (long long)(h0 + g) * HD + 16 * t;
+    float f[32], top = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float a[8];
-        unpack8<T>(*reinterpret_cast<const int4*>(qp + 64 * i), a);
+    for (int i = 0; i < 4; ++i) {
+      float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (g < nh) unpack8<T>(*reinterpret_cast<const int4*>(reinterpret_cast<const T*>(p.q) + b * p.q_ld + (long long)(h0 + g) * HD + 32 * t + 8 * i), a);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[i][j] = a[j];
-        unpack8<T>(*reinterpret_cast<const int4*>(qp + 64 * i + 8), a);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[i][8 + j] = a[j];
+      for (int j = 0; j < 8; ++j) {
+        f[8 * i + j] = a[j];
+        top = fmaxf(top, fabsf(a[j]));
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(f[i][j]));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) f[i][j] = 0.f;
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -345,93 +405,67 @@ __global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
     const float up = pow2i(14 - e);
     fq = p.scale_log2 * pow2i(e - 14);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        aq[4 * i + w][0] = Cvt<__half>::pack2(f[i][4 * w] * up, f[i][4 * w + 1] * up);
-        aq[4 * i + w][1] = Cvt<__half>::pack2(f[i][4 * w + 2] * up, f[i][4 * w + 3] * up);
-      }
+    for (int s = 0; s < 8; ++s) {
+      aq[s][0] = Cvt<__half>::pack2(f[4 * s] * up, f[4 * s + 1] * up);
+      aq[s][1] = Cvt<__half>::pack2(f[4 * s + 2] * up, f[4 * s + 3] * up);
+    }
   }
 
-  const int* table = p.tables + (long long)b * p.max_blocks;
-  // pages of a tile's halves; a half that begins at or after the end has none
-  auto pages = [&](int at, int (&pg)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int tb = at * 16 + 8 * h;
-      pg[h] = at < end && tb < ctx ? table[(uint32_t)tb / (uint32_t)p.bs] : -1;
-    }
-  };
-  auto fetch = [&](int at, const int (&pg)[2], Tile& x) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (pg[h] >= 0) {
-        const long long sc = (long long)pg[h] * p.KV + kvh;
-        const uint32_t off = (uint32_t)(at * 16 + 8 * h) % (uint32_t)p.bs;
-        const long long base = (sc * p.bs + off) * HD;
-        const uint8_t* kp = p.k8 + base + g * HD + 16 * t;
-        const uint8_t* vp = p.v8 + base + 2 * t * HD + 16 * g;
-        x.k[h][0] = ld_nc_v4(kp);
-        x.k[h][1] = ld_nc_v4(kp + 64);
-        x.v[h][0] = ld_nc_v4(vp);
-        x.v[h][1] = ld_nc_v4(vp + HD);
-        x.ks[h] = p.ks[sc];
-        x.vs[h] = p.vs[sc];
-      } else {
-        x.k[h][0] = x.k[h][1] = x.v[h][0] = x.v[h][1] = make_int4(0, 0, 0, 0);
-        x.ks[h] = 1.f;
-        x.vs[h] = pow2i(E_LOW);
-      }
-    }
-  };
-
-  float m = -INFINITY, l = 0.f, vref = pow2i(E_LOW);
+  float m = -INFINITY, l = 0.f, vref = pow2i(E_LOW), vinv = pow2i(-E_LOW);
   float o[16][4];
 #pragma unroll
   for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
-  int pg[2];
-  Tile nx;
-  pages(tile, pg);
-  fetch(tile, pg, nx);
-  pages(tile + NW, pg);
+  int slot = 0;
   for (; tile < end; tile += NW) {
-    Tile x = nx;
-    fetch(tile + NW, pg, nx);
-    pages(tile + 2 * NW, pg);
+    asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
+    __syncwarp();                                           // this tile is there for every lane, and every lane has read the one before it
+    const uint32_t kv = ring + slot * (uint32_t)sizeof(Stage);
+    const float4 sc = *reinterpret_cast<const float4*>(&s_scale[warp][slot][0]);
+    {
+      const int ahead = slot == 0 ? RING - 1 : slot - 1;
+      fill(tile + (RING - 1) * NW, pg, ahead);
+      pages(tile + RING * NW, pg);
+    }
+    slot = slot == RING - 1 ? 0 : slot + 1;
+    const float ksc[2] = {sc.x, sc.y}, vsc[2] = {sc.z, sc.w};
     float z[2][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const uint32_t w = word(x.k[h][s >> 2], s & 3);
-        mma_f16(c, aq[s][0], 0u, aq[s][1], 0u, half2_of_e4m3x2(w & 0xffffu), half2_of_e4m3x2(w >> 16));
+      for (int i = 0; i < 2; ++i) {
+        const int4 k = lds128(kv + (8 * h + g) * 128 + ((2 * t + i) ^ g) * 16);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t b0, b1;
+          half4_of_e4m3x4(word(k, w), b0, b1);
+          mma_f16(c, aq[4 * i + w][0], 0u, aq[4 * i + w][1], 0u, b0, b1);
+        }
       }
-      const float f = fq * x.ks[h];
+      const float f = fq * ksc[h];
       z[h][0] = c[0] * f;
       z[h][1] = c[1] * f;
     }
+    const int left = ctx - tile * 16 - 2 * t;               // tokens 2t + 8h + i are there while 8h + i < left
     const bool edge = tile * 16 + 16 > ctx;
-    if (edge) {                                            // tokens behind the end: no weight, and whatever the page holds there is no value
+    if (edge) {                                             // tokens behind the end have no weight
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          if (tile * 16 + 8 * h + 2 * t + i >= ctx) {
-            z[h][i] = -INFINITY;
-            x.v[h][i] = make_int4(0, 0, 0, 0);
-          }
+          if (8 * h + i >= left) z[h][i] = -INFINITY;
     }
     float mx = fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float vnew = fmaxf(vref, fmaxf(x.vs[0], x.vs[1]));
+    const float vnew = fmaxf(vref, fmaxf(vsc[0], vsc[1]));
     if (__any_sync(0xffffffffu, mx > m) || vnew > vref) {
       const float mn = fmaxf(m, mx);
       const float a = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2f(m - mn);
       l *= a;
-      const float ao = a * (vref / vnew);
+      vinv = 1.f / vnew;
+      const float ao = a * (vref * vinv);
       m = mn;
       vref = vnew;
 #pragma unroll
@@ -446,37 +480,45 @@ __global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float p0 = ex2f(z[h][0] - m), p1 = ex2f(z[h][1] - m);
-      if (edge) {                                          // m may be -inf itself
-        if (tile * 16 + 8 * h + 2 * t >= ctx) p0 = 0.f;
-        if (tile * 16 + 8 * h + 2 * t + 1 >= ctx) p1 = 0.f;
+      if (edge) {                                           // m may be -inf itself
+        if (8 * h >= left) p0 = 0.f;
+        if (8 * h + 1 >= left) p1 = 0.f;
       }
       l += p0 + p1;
-      const float f = x.vs[h] / vref * P_UNIT;
-      const __half2 a = __floats2half2_rn(p0 * f, p1 * f);
+      const float f = vsc[h] * vinv * P_UNIT;               // powers of two
+      p0 *= f;
+      p1 *= f;
+      const __half2 a = __floats2half2_rn(p0, p1);
       const float2 r = __half22float2(a);
-      const __half2 c = __floats2half2_rn(p0 * f - r.x, p1 * f - r.y);
+      const __half2 c = __floats2half2_rn(p0 - r.x, p1 - r.y);
       hi[h] = *reinterpret_cast<const uint32_t*>(&a);
       lo[h] = *reinterpret_cast<const uint32_t*>(&c);
     }
+    int4 v[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v[h][i] = lds128(kv + 16 * 128 + (8 * h + 2 * t + i) * 128 + (g ^ (2 * t + i)) * 16);
+        if (edge && 8 * h + i >= left) v[h][i] = make_int4(0, 0, 0, 0);      // whatever a page holds behind the end is no value
+      }
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      uint32_t e[2], f[2];
+      uint32_t b[2][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        e[h] = __byte_perm(word(x.v[h][0], w), word(x.v[h][1], w), 0x5140);
-        f[h] = __byte_perm(word(x.v[h][0], w), word(x.v[h][1], w), 0x7362);
+        half4_of_e4m3x4(__byte_perm(word(v[h][0], w), word(v[h][1], w), 0x5140), b[h][0], b[h][1]);
+        half4_of_e4m3x4(__byte_perm(word(v[h][0], w), word(v[h][1], w), 0x7362), b[h][2], b[h][3]);
       }
-      mma_f16(o[4 * w], hi[0], lo[0], hi[1], lo[1], half2_of_e4m3x2(e[0] & 0xffffu), half2_of_e4m3x2(e[1] & 0xffffu));
-      mma_f16(o[4 * w + 1], hi[0], lo[0], hi[1], lo[1], half2_of_e4m3x2(e[0] >> 16), half2_of_e4m3x2(e[1] >> 16));
-      mma_f16(o[4 * w + 2], hi[0], lo[0], hi[1], lo[1], half2_of_e4m3x2(f[0] & 0xffffu), half2_of_e4m3x2(f[1] & 0xffffu));
-      mma_f16(o[4 * w + 3], hi[0], lo[0], hi[1], lo[1], half2_of_e4m3x2(f[0] >> 16), half2_of_e4m3x2(f[1] >> 16));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mma_f16(o[4 * w + i], hi[0], lo[0], hi[1], lo[1], b[0][i], b[1][i]);
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 
   // join the warps: lane (g, t) holds dimensions 32 t .. 32 t + 31 of head g
-  constexpr int PITCH = HD + 4;
-  __shared__ float s_o[NW][8][PITCH];
-  __shared__ float s_m[NW][8], s_l[NW][8];
+  __syncthreads();                                          // the rings are done with
+  auto& s_o = sm.o;
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
   {
@@ -537,7 +579,14 @@ __global__ void __launch_bounds__(HD) join8_kernel(const float* __restrict__ par
 template <typename T>
 int attend8_t(const Attend8& p, int batch, cudaStream_t st) {
   const int H = p.G * p.KV;
-  DLTI_CUDA_CHECK(dlti_launch_pdl(batch, attend8_kernel<T>, dim3(p.splits, p.KV * ((p.G + 7) / 8), batch), dim3(32 * NW), 0, st, p));
+  static bool set[64] = {};                       // the attribute is per device
+  int dev = 0;
+  DLTI_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!set[dev & 63]) {
+    DLTI_CUDA_CHECK(cudaFuncSetAttribute(attend8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(AttendSmem)));
+    set[dev & 63] = true;
+  }
+  DLTI_CUDA_CHECK(dlti_launch_pdl(batch, attend8_kernel<T>, dim3(p.splits, p.KV * ((p.G + 7) / 8), batch), dim3(32 * NW), sizeof(AttendSmem), st, p));
   if (p.splits > 1)
     DLTI_CUDA_CHECK(dlti_launch_pdl(batch, join8_kernel<T>, dim3(H, batch), dim3(HD), 0, st, (const float*)p.part_o, (const float*)p.part_ml,
                                     p.splits, (T*)p.out, p.out_ld));
@@ -618,7 +667,7 @@ DLTI_API int dlti_paged_decode8(const void* q, long long q_ld, const void* k8, c
   if (!sizes_ok("paged_decode8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
   if (batch <= 0) return 0;
   if (batch > 65535 || splits < 1 || (splits > 1 && !workspace)) return DLTI_ERR_BAD_ARG;
-  const Attend8 p{q, q_ld, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, tables, ctx, max_blocks, bs, H / KV, KV, splits,
+  const Attend8 p{q, q_ld, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, tables, ctx, max_blocks, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs), H / KV, KV, splits,
                   scale * 1.4426950408889634f, workspace, workspace + (long long)batch * H * splits * HD, out, out_ld};
   if (dtype == DLTI_BF16) return attend8_t<__nv_bfloat16>(p, batch, st);
   if (dtype == DLTI_FP16) return attend8_t<__half>(p, batch, st);
