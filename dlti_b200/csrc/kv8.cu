@@ -7,6 +7,7 @@
 #include "common.cuh"
 
 #include <cstdio>
+#include <type_traits>
 
 namespace {
 
@@ -283,6 +284,7 @@ __device__ __forceinline__ uint32_t word(const int4& v, int i) { return (uint32_
 constexpr int NW = 4;            // warps of a CTA
 constexpr int RING = 3;          // tiles of a warp in flight or in use
 constexpr float P_UNIT = 32768.f;
+constexpr int MAX_PARTS = 16;
 
 struct __align__(128) Stage {
   uint8_t k[16][128], v[16][128];
@@ -302,11 +304,11 @@ __device__ __forceinline__ int4 lds128(uint32_t a) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int n) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, int n) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
 struct Attend8 {
@@ -315,18 +317,53 @@ struct Attend8 {
   const uint8_t *k8, *v8;
   const float *ks, *vs;
   const int *tables, *ctx;
-  int max_blocks, bs, shift, G, KV, splits;      // shift: bs = 1 << shift, or -1
+  int max_blocks, bs, shift, G, KV, splits, parts;      // shift: bs = 1 << shift, or -1; parts: clusters of a context
   float scale_log2;
-  float *part_o, *part_ml;       // [batch, heads, splits, 128], [..., 2]
+  float *part_o, *part_ml;       // [batch, heads, parts, 128], [..., 2]
   void* out;
   long long out_ld;
 };
 
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote(uint32_t a, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float remote_f(uint32_t a, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote(a, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 remote_f2(uint32_t a, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote(a, rank)) : "memory");
+  return v;
+}
+// factor of a part with maximum m and sum l among parts of maximum top; a part without tokens has m = -inf and l = 0
+__device__ __forceinline__ float share(float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2f(m - top); }
 template <typename T>
-__global__ void __launch_bounds__(32 * NW, 4) attend8_kernel(const Attend8 p) {
+__device__ __forceinline__ void finish(const Attend8& p, T* out, int b, int head, int d, float acc, float sum, float top, int part) {
+  if (p.parts == 1) {
+    out[b * p.out_ld + (long long)head * HD + d] = Cvt<T>::from_f(sum == 0.f ? 0.f : acc / sum);
+  } else {
+    const long long at = ((long long)b * (p.G * p.KV) + head) * p.parts + part;
+    p.part_o[at * HD + d] = acc;
+    if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(top, sum);
+  }
+}
+
+// WHOLE: a tile lies in one page (block_size a multiple of 16)
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
   extern __shared__ __align__(128) unsigned char raw[];
   AttendSmem& sm = *reinterpret_cast<AttendSmem*>(raw);
   __shared__ float s_m[NW][8], s_l[NW][8];
+  __shared__ float2 s_cml[8];
   __shared__ __align__(16) float s_scale[NW][RING][4];      // of a tile's halves: keys, values
   griddep_pass(gridDim.z);
   const int split = blockIdx.x, b = blockIdx.z;
@@ -343,36 +380,48 @@ __global__ void __launch_bounds__(32 * NW, 4) attend8_kernel(const Attend8 p) {
   // ---- the ring
   const int* table = p.tables + (long long)b * p.max_blocks;
   const uint32_t ring = smem_u32(&sm.ring[warp][0]), scales = smem_u32(&s_scale[warp][0][0]);
-  const int r8 = lane >> 3, c16 = (lane & 7) * 16;          // a lane copies bytes c16 .. of rows r8, r8 + 4, ... of a tile
+  // a lane copies 16 bytes of rows r8, r8 + 4 of both halves
+  const int r8 = lane >> 3, c16 = (lane & 7) * 16;
+  const uint8_t* kl = p.k8 + r8 * HD + c16;
+  const uint8_t* vl = p.v8 + r8 * HD + c16;
+  const uint32_t to0 = ring + r8 * 128 + (c16 ^ (r8 << 4)), to1 = ring + (r8 + 4) * 128 + (c16 ^ (r8 + 4) << 4);
+  const bool sv = lane & 1;                                 // lanes 0 .. 3 bring the scales: keys, values of the halves
+  const float* sl = sv ? p.vs : p.ks;
+  const uint32_t sto = scales + (2 * sv + (lane >> 1)) * 4;
   auto page_at = [&](int tb) { return p.shift >= 0 ? tb >> p.shift : (int)((uint32_t)tb / (uint32_t)p.bs); };
-  // pages of a tile's halves; a half that begins at or after the end has none
+  // pages of a tile's halves. A half that begins behind the end takes the first half's rows: it has no weight
   auto pages = [&](int at, int (&pg)[2]) {
-    const int tb = at * 16;
-    pg[0] = at < end ? table[page_at(tb)] : -1;
-    pg[1] = at < end && tb + 8 < ctx ? table[page_at(tb + 8)] : -1;
+    if (at < end) {
+      pg[0] = table[page_at(at * 16)];
+      if (!WHOLE) pg[1] = at * 16 + 8 < ctx ? table[page_at(at * 16 + 8)] : -1;
+    }
   };
   auto fill = [&](int at, const int (&pg)[2], int slot) {
     if (at < end) {
-      const uint32_t dst = ring + slot * (uint32_t)sizeof(Stage);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bool ok = pg[h] >= 0;
-        const long long sc = ok ? (long long)pg[h] * p.KV + kvh : 0;
-        const int tb = at * 16 + 8 * h, off = tb - page_at(tb) * p.bs;
-        const long long base = ok ? (sc * p.bs + off) * HD + r8 * HD + c16 : 0;
-        const int n = ok ? 16 : 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = r8 + 4 * i;
-          const uint32_t d = dst + (8 * h + r) * 128 + (c16 ^ (r << 4));
-          cp16(d, p.k8 + base + i * 4 * HD, n);
-          cp16(d + 16 * 128, p.v8 + base + i * 4 * HD, n);
-        }
-        if ((lane >> 1) == h) {                             // lanes 2 h, 2 h + 1: this half's scales
-          const bool v = lane & 1;
-          cp4(scales + (slot * 4 + 2 * v + h) * 4, (v ? p.vs : p.ks) + sc, ok ? 4 : 0);
+      const uint32_t s = slot * (uint32_t)sizeof(Stage);
+      uint32_t head[2], row[2];                             // page and head; row of the cache
+      const int tb = at * 16;
+      head[0] = (uint32_t)pg[0] * p.KV + kvh;
+      row[0] = head[0] * p.bs + (tb - page_at(tb) * p.bs);
+      head[1] = head[0];
+      row[1] = row[0] + 8;
+      if (!WHOLE) {
+        if (pg[1] >= 0) {
+          head[1] = (uint32_t)pg[1] * p.KV + kvh;
+          row[1] = head[1] * p.bs + (tb + 8 - page_at(tb + 8) * p.bs);
+        } else {
+          row[1] = row[0];
         }
       }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned long long at_row = (unsigned long long)row[h] * HD;
+        cp16(to0 + s + h * 1024, kl + at_row);
+        cp16(to1 + s + h * 1024, kl + at_row + 4 * HD);
+        cp16(to0 + s + h * 1024 + 2048, vl + at_row);
+        cp16(to1 + s + h * 1024 + 2048, vl + at_row + 4 * HD);
+      }
+      if (lane < 4) cp4(sto + slot * 16, sl + head[lane >> 1]);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -417,7 +466,8 @@ __global__ void __launch_bounds__(32 * NW, 4) attend8_kernel(const Attend8 p) {
   for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
   int slot = 0;
-  for (; tile < end; tile += NW) {
+  auto step = [&](auto last) {
+    constexpr bool edge = decltype(last)::value;            // some tokens of the tile are behind the end
     asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
     __syncwarp();                                           // this tile is there for every lane, and every lane has read the one before it
     const uint32_t kv = ring + slot * (uint32_t)sizeof(Stage);
@@ -448,8 +498,7 @@ __global__ void __launch_bounds__(32 * NW, 4) attend8_kernel(const Attend8 p) {
       z[h][1] = c[1] * f;
     }
     const int left = ctx - tile * 16 - 2 * t;               // tokens 2t + 8h + i are there while 8h + i < left
-    const bool edge = tile * 16 + 16 > ctx;
-    if (edge) {                                             // tokens behind the end have no weight
+    if constexpr (edge) {                                   // tokens behind the end have no weight
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -480,7 +529,7 @@ __global__ void __launch_bounds__(32 * NW, 4) attend8_kernel(const Attend8 p) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float p0 = ex2f(z[h][0] - m), p1 = ex2f(z[h][1] - m);
-      if (edge) {                                           // m may be -inf itself
+      if constexpr (edge) {                                 // m may be -inf itself
         if (8 * h >= left) p0 = 0.f;
         if (8 * h + 1 >= left) p1 = 0.f;
       }
@@ -500,7 +549,8 @@ __global__ void __launch_bounds__(32 * NW, 4) attend8_kernel(const Attend8 p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         v[h][i] = lds128(kv + 16 * 128 + (8 * h + 2 * t + i) * 128 + (g ^ (2 * t + i)) * 16);
-        if (edge && 8 * h + i >= left) v[h][i] = make_int4(0, 0, 0, 0);      // whatever a page holds behind the end is no value
+        if constexpr (edge)                                 // whatever a page holds behind the end is no value
+          if (8 * h + i >= left) v[h][i] = make_int4(0, 0, 0, 0);
       }
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -513,7 +563,11 @@ __global__ void __launch_bounds__(32 * NW, 4) attend8_kernel(const Attend8 p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) mma_f16(o[4 * w + i], hi[0], lo[0], hi[1], lo[1], b[0][i], b[1][i]);
     }
-  }
+    tile += NW;
+  };
+  const int whole = min(end, ctx / 16);
+  while (tile < whole) step(std::false_type{});
+  if (tile < end) step(std::true_type{});
   asm volatile("cp.async.wait_all;" ::: "memory");
 
   // join the warps: lane (g, t) holds dimensions 32 t .. 32 t + 31 of head g
@@ -537,60 +591,98 @@ __global__ void __launch_bounds__(32 * NW, 4) attend8_kernel(const Attend8 p) {
     }
   }
   __syncthreads();
+  // Splits of one context are a cluster of up to 8 CTAs that join through distributed shared memory; with more, each cluster's sum goes to the
+  // workspace.
+  const uint32_t crank = cluster_rank(), csize = cluster_size();
+  const int d = threadIdx.x;
   for (int h = 0; h < nh; ++h) {
     float gm = s_m[0][h], gl = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 1; w < NW; ++w) gm = fmaxf(gm, s_m[w][h]);
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float mw = s_m[w][h], lw = s_l[w][h];
-      const float a = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2f(mw - gm);
-      gl += lw * a;
-      acc += s_o[w][h][threadIdx.x] * a;
+      const float a = share(s_m[w][h], s_l[w][h], gm);
+      gl += s_l[w][h] * a;
+      acc += s_o[w][h][d] * a;
     }
-    const long long row = (long long)b * (p.G * p.KV) + h0 + h;
-    if (p.splits == 1) {
-      reinterpret_cast<T*>(p.out)[b * p.out_ld + (long long)(h0 + h) * HD + threadIdx.x] = Cvt<T>::from_f(gl == 0.f ? 0.f : acc / gl);
+    if (csize == 1) {
+      finish(p, reinterpret_cast<T*>(p.out), b, h0 + h, d, acc, gl, gm, split);
     } else {
-      p.part_o[(row * p.splits + split) * HD + threadIdx.x] = acc;
-      if (threadIdx.x == 0) *reinterpret_cast<float2*>(p.part_ml + (row * p.splits + split) * 2) = make_float2(gm, gl);
+      s_o[0][h][d] = acc;                                   // nobody else reads column d
+      if (d == 0) s_cml[h] = make_float2(gm, gl);
     }
   }
+  if (csize == 1) return;
+  cluster_barrier();
+  for (int h = crank; h < nh; h += csize) {
+    const uint32_t ml = smem_u32(&s_cml[h]), at = smem_u32(&s_o[0][h][d]);
+    float2 x[8];
+    float v[8], gm = -INFINITY, gl = 0.f, acc = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < (int)csize) {
+        x[c] = remote_f2(ml, c);
+        v[c] = remote_f(at, c);
+      }
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < (int)csize) gm = fmaxf(gm, x[c].x);
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < (int)csize) {
+        const float a = share(x[c].x, x[c].y, gm);
+        gl += x[c].y * a;
+        acc += v[c] * a;
+      }
+    finish(p, reinterpret_cast<T*>(p.out), b, h0 + h, d, acc, gl, gm, split / (int)csize);
+  }
+  cluster_barrier();                                        // shared memory stays until everyone has read it
 }
 
 template <typename T>
-__global__ void __launch_bounds__(HD) join8_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, int splits,
+__global__ void __launch_bounds__(HD) join8_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, int parts,
                                                    T* __restrict__ out, long long out_ld) {
   griddep_pass(gridDim.y);
   const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const long long at = ((long long)b * gridDim.x + h) * splits;
-  float gm = -INFINITY;
-  for (int s = 0; s < splits; ++s) gm = fmaxf(gm, part_ml[(at + s) * 2]);
-  float acc = 0.f, gl = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(part_ml + (at + s) * 2);
-    const float a = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2f(ml.x - gm);
-    gl += ml.y * a;
-    acc += part_o[(at + s) * HD + d] * a;
-  }
+  const long long at = ((long long)b * gridDim.x + h) * parts;
+  float gm = -INFINITY, acc = 0.f, gl = 0.f;
+  float v[MAX_PARTS];
+  float2 x[MAX_PARTS];
+#pragma unroll
+  for (int s = 0; s < MAX_PARTS; ++s)
+    if (s < parts) {
+      x[s] = *reinterpret_cast<const float2*>(part_ml + (at + s) * 2);
+      v[s] = part_o[(at + s) * HD + d];
+      gm = fmaxf(gm, x[s].x);
+    }
+#pragma unroll
+  for (int s = 0; s < MAX_PARTS; ++s)
+    if (s < parts) {
+      const float a = share(x[s].x, x[s].y, gm);
+      gl += x[s].y * a;
+      acc += v[s] * a;
+    }
   out[b * out_ld + (long long)h * HD + d] = Cvt<T>::from_f(gl == 0.f ? 0.f : acc / gl);
 }
 
 template <typename T>
 int attend8_t(const Attend8& p, int batch, cudaStream_t st) {
   const int H = p.G * p.KV;
+  const bool whole = p.bs % 16 == 0;
   static bool set[64] = {};                       // the attribute is per device
   int dev = 0;
   DLTI_CUDA_CHECK(cudaGetDevice(&dev));
   if (!set[dev & 63]) {
-    DLTI_CUDA_CHECK(cudaFuncSetAttribute(attend8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(AttendSmem)));
+    DLTI_CUDA_CHECK(cudaFuncSetAttribute(attend8_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(AttendSmem)));
+    DLTI_CUDA_CHECK(cudaFuncSetAttribute(attend8_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(AttendSmem)));
     set[dev & 63] = true;
   }
-  DLTI_CUDA_CHECK(dlti_launch_pdl(batch, attend8_kernel<T>, dim3(p.splits, p.KV * ((p.G + 7) / 8), batch), dim3(32 * NW), sizeof(AttendSmem), st, p));
-  if (p.splits > 1)
+  DLTI_CUDA_CHECK(dlti_launch_pdl_cluster(batch, p.splits / p.parts, whole ? attend8_kernel<T, true> : attend8_kernel<T, false>,
+                                          dim3(p.splits, p.KV * ((p.G + 7) / 8), batch), dim3(32 * NW), sizeof(AttendSmem), st, p));
+  if (p.parts > 1)
     DLTI_CUDA_CHECK(dlti_launch_pdl(batch, join8_kernel<T>, dim3(H, batch), dim3(HD), 0, st, (const float*)p.part_o, (const float*)p.part_ml,
-                                    p.splits, (T*)p.out, p.out_ld));
-  dlti_count_launch(p.splits > 1 ? 2 : 1);
+                                    p.parts, (T*)p.out, p.out_ld));
+  dlti_count_launch(p.parts > 1 ? 2 : 1);
   return 0;
 }
 
@@ -657,18 +749,20 @@ DLTI_API int dlti_acc_rope_cache8(float* acc, void* out, long long out_ld, const
   return DLTI_ERR_UNSUPPORTED;
 }
 
-// floats of workspace that dlti_paged_decode8 needs with more than one split
-DLTI_API long long dlti_paged_decode8_floats(int batch, int H, int splits) { return splits > 1 ? (long long)batch * H * splits * (HD + 2) : 0; }
+// floats of workspace that dlti_paged_decode8 needs: none for up to 8 splits, which are one cluster
+DLTI_API long long dlti_paged_decode8_floats(int batch, int H, int splits) { return splits > 8 ? (long long)batch * H * ((splits + 7) / 8) * (HD + 2) : 0; }
 
-// q [batch, q_ld] (head h at column h * 128) -> out [batch, out_ld]; contexts of 0 give zeros.
+// q [batch, q_ld] (head h at column h * 128) -> out [batch, out_ld]; contexts of 0 give zeros. splits: 1 .. 128, the same number in each of
+// ceil(splits / 8) clusters.
 DLTI_API int dlti_paged_decode8(const void* q, long long q_ld, const void* k8, const void* v8, const float* ks, const float* vs,
                                 const int* tables, int max_blocks, const int* ctx, int batch, int bs, int H, int KV, int hd, float scale,
                                 int splits, float* workspace, void* out, long long out_ld, int dtype, cudaStream_t st) {
   if (!sizes_ok("paged_decode8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
   if (batch <= 0) return 0;
-  if (batch > 65535 || splits < 1 || (splits > 1 && !workspace)) return DLTI_ERR_BAD_ARG;
-  const Attend8 p{q, q_ld, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, tables, ctx, max_blocks, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs), H / KV, KV, splits,
-                  scale * 1.4426950408889634f, workspace, workspace + (long long)batch * H * splits * HD, out, out_ld};
+  const int parts = (splits + 7) / 8;
+  if (batch > 65535 || splits < 1 || parts > MAX_PARTS || splits % parts || (parts > 1 && !workspace)) return DLTI_ERR_BAD_ARG;
+  const Attend8 p{q, q_ld, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, tables, ctx, max_blocks, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs),
+                  H / KV, KV, splits, parts, scale * 1.4426950408889634f, workspace, workspace + (long long)batch * H * parts * HD, out, out_ld};
   if (dtype == DLTI_BF16) return attend8_t<__nv_bfloat16>(p, batch, st);
   if (dtype == DLTI_FP16) return attend8_t<__half>(p, batch, st);
   return DLTI_ERR_UNSUPPORTED;

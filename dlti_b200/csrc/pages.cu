@@ -55,23 +55,25 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
 
 }  // namespace
 
-// caches: base addresses; layers, layer_bytes, page_stride, page_bytes: of each. Pages from[i] -> to[i] of every layer of every cache, on the host;
-// no page is written twice or both read and written (the caller's check).
-DLTI_API int dlti_copy_pages(void* const* bases, const int* layers, const long long* layer_bytes, const long long* page_stride,
-                             const long long* page_bytes, int caches, const int* from, const int* to, int pairs, cudaStream_t st) {
-  if (pairs <= 0 || caches <= 0) return 0;
-  for (int c = 0; c < caches; ++c)
-    if (page_bytes[c] <= 0 || page_bytes[c] > 1 << 30 || layers[c] <= 0) {
-      dlti_set_error("copy_pages: a cache without layers or with pages of no or more than 2^30 bytes");
+// caches: base address, layers, bytes from layer to layer, bytes from page to page, bytes of a page, of each. Pages from[i] -> to[i] of every
+// layer of every cache, all on the host; no page is written twice or both read and written (the caller's check).
+DLTI_API int dlti_copy_pages(const long long* caches, int count, const int* from, const int* to, int pairs, cudaStream_t st) {
+  if (pairs <= 0 || count <= 0) return 0;
+  for (int c = 0; c < count; ++c) {
+    const long long layers = caches[5 * c + 1], bytes = caches[5 * c + 4];
+    if (bytes <= 0 || bytes > 1 << 30 || layers <= 0 || layers * ((bytes + PIECE - 1) / PIECE) > 1 << 24) {
+      dlti_set_error("copy_pages: a cache without layers, with pages of nothing, or with more than 2^24 pieces of 16 KB in a page of all layers");
       return DLTI_ERR_BAD_ARG;
     }
+  }
   CopyJob job;
-  for (int c0 = 0; c0 < caches; c0 += MAX_CACHES) {
-    job.caches = caches - c0 < MAX_CACHES ? caches - c0 : MAX_CACHES;
+  for (int c0 = 0; c0 < count; c0 += MAX_CACHES) {
+    job.caches = count - c0 < MAX_CACHES ? count - c0 : MAX_CACHES;
     job.first[0] = 0;
     for (int c = 0; c < job.caches; ++c) {
-      job.cache[c] = Cache{(char*)bases[c0 + c], layer_bytes[c0 + c], page_stride[c0 + c], layers[c0 + c], (int)page_bytes[c0 + c]};
-      job.first[c + 1] = job.first[c] + layers[c0 + c] * (int)((page_bytes[c0 + c] + PIECE - 1) / PIECE);
+      const long long* k = caches + 5 * (c0 + c);
+      job.cache[c] = Cache{reinterpret_cast<char*>(k[0]), k[2], k[3], (int)k[1], (int)k[4]};
+      job.first[c + 1] = job.first[c] + (int)k[1] * (int)((k[4] + PIECE - 1) / PIECE);
     }
     for (int p0 = 0; p0 < pairs; p0 += MAX_PAIRS) {
       const int n = pairs - p0 < MAX_PAIRS ? pairs - p0 : MAX_PAIRS;

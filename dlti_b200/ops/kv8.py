@@ -28,32 +28,63 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _cache_fits(k8, v8, k_scale, v_scale, H: int, KV: int, hd: int) -> bool:
+    s = k8.shape
+    return (len(s) == 4 and s == v8.shape and s[1] == KV and s[3] == hd and s[2] >= 8 and s[2] % 8 == 0 and KV > 0 and H > 0 and H % KV == 0
+            and k8.dtype is E4M3 and v8.dtype is E4M3 and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
+            and k_scale.shape == v_scale.shape == s[:2] and k8.is_contiguous() and v8.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous() and s[0] * s[2] < 1 << 31)
+
+
 def _check_cache(op: str, k8, v8, k_scale, v_scale, H: int, KV: int, hd: int) -> None:
+    if _cache_fits(k8, v8, k_scale, v_scale, H, KV, hd):
+        return
     _need(k8.dim() == 4 and k8.shape == v8.shape and k8.shape[1] == KV and k8.shape[3] == hd,
           f"{op}: pages are [num_blocks, {KV}, block_size, {hd}], got {tuple(k8.shape)} and {tuple(v8.shape)}")
     _need(KV > 0 and H > 0 and H % KV == 0, f"{op}: query heads are a multiple of key/value heads, got {H} and {KV}")
     _need(k8.dtype == v8.dtype == E4M3 and k_scale.dtype == v_scale.dtype == torch.float32, f"{op}: pages are float8_e4m3fn with float32 scales")
     _need(k_scale.shape == v_scale.shape == k8.shape[:2], f"{op}: one scale for each page and head")
-    _need(k8.is_contiguous() and v8.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous(), f"{op}: pages and scales are contiguous")
     _need(k8.shape[2] >= 8 and k8.shape[2] % 8 == 0, f"{op}: block_size is a multiple of 8, got {k8.shape[2]}")
     _need(k8.shape[0] * k8.shape[2] < 1 << 31, f"{op}: slots have 31 bits")
+    raise ValueError(f"{op}: pages and scales are contiguous")
 
 
-def _check_device(op: str, *tensors) -> None:
+def _check_device(op: str, *tensors) -> int:
+    """The current device, which every tensor is on."""
     d = torch.cuda.current_device()
     for t in tensors:
-        _need(t.is_cuda and t.device.index == d, f"{op}: every tensor is on the current device, cuda:{d}")
+        if t.get_device() != d:
+            raise ValueError(f"{op}: every tensor is on the current device, cuda:{d}")
+    return d
 
 
 def _check_rows(op: str, x, width: int) -> None:
-    _need(x.dim() == 2 and x.shape[1] == width and x.stride(1) == 1, f"{op}: rows [tokens, {width}] with consecutive columns")
-    _need(x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0, f"{op}: rows begin at multiples of 16 bytes")
+    s = x.stride()
+    if len(s) != 2 or x.shape[1] != width or s[1] != 1:
+        raise ValueError(f"{op}: rows [tokens, {width}] with consecutive columns")
+    if s[0] % 8 or x.data_ptr() % 16:
+        raise ValueError(f"{op}: rows begin at multiples of 16 bytes")
+
+
+def _check_places(op: str, pos, slots, T: int) -> None:
+    if not (pos.dtype is torch.int32 and slots.dtype is torch.int64 and pos.shape == slots.shape == (T,) and pos.is_contiguous()
+            and slots.is_contiguous()):
+        raise ValueError(f"{op}: a position (int32) and a slot (int64) for each row")
+
+
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_bound: dict = {}
+
+
+def _fn(name: str, types: tuple):
+    f = _bound.get(name)
+    if f is None:
+        f = _bound[name] = _lib.fn(name, list(types))
+    return f
 
 
 def _check_slots(op: str, slots, bs: int, num_blocks: int) -> None:
     """Only with the opt-in checks: slots inside the cache, each once, rows of one page next to one another."""
-    if not _debug.ENABLED:
-        return
     _debug.check_range(op, "slots", slots, 0, num_blocks * bs, allow=-1)
     s = slots.to("cpu")
     s = s[s >= 0]
@@ -110,28 +141,31 @@ def rope_cache8_(qkv, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV,
     dst = qkv if out is None else out
     bs = k8.shape[2]
     _check_cache("rope_cache8", k8, v8, k_scale, v_scale, H, KV, hd)
-    _check_slots("rope_cache8", slots, bs, k8.shape[0])
-    _debug.check_range("rope_cache8", "positions", pos, 0, cos_t.shape[0])
+    if _debug.ENABLED:
+        _check_slots("rope_cache8", slots, bs, k8.shape[0])
+        _debug.check_range("rope_cache8", "positions", pos, 0, cos_t.shape[0])
     T, W = qkv.shape[0], (H + 2 * KV) * hd
-    _need(dst.shape == qkv.shape and dst.dtype == qkv.dtype, "rope_cache8: out has the shape and type of the rows")
-    _need(pos.shape == slots.shape == (T,) and pos.dtype == torch.int32 and slots.dtype == torch.int64 and pos.is_contiguous() and slots.is_contiguous(),
-          "rope_cache8: a position (int32) and a slot (int64) for each row")
-    if not _lib.use_native(qkv):
+    if out is not None:
+        _need(dst.shape == qkv.shape and dst.dtype == qkv.dtype, "rope_cache8: out has the shape and type of the rows")
+    _check_places("rope_cache8", pos, slots, T)
+    if not qkv.is_cuda:
         return rope_cache8_ref(qkv, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV, hd, out)
-    _check_device("rope_cache8", qkv, dst, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale)
+    dev = _check_device("rope_cache8", qkv, dst, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale)
     _check_rows("rope_cache8", qkv, W)
-    _check_rows("rope_cache8", dst, W)
+    if out is not None:
+        _check_rows("rope_cache8", dst, W)
     _check_tables(cos_t, sin_t, hd)
-    f = _lib.fn("dlti_rope_cache8", [_V, _L, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V])
+    f = _fn("dlti_rope_cache8", (_V, _L, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V))
     _lib.check(f(qkv.data_ptr(), qkv.stride(0), dst.data_ptr(), dst.stride(0), pos.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), slots.data_ptr(),
                  k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), T, H, KV, hd, bs, _lib.dtype_code(qkv.dtype),
-                 _lib.stream_ptr()), "rope_cache8")
+                 _stream(dev)), "rope_cache8")
     return dst
 
 
 def _check_tables(cos_t, sin_t, hd: int) -> None:
-    _need(cos_t.shape == sin_t.shape and cos_t.shape[1] == hd // 2 and cos_t.dtype == sin_t.dtype == torch.float32 and cos_t.is_contiguous()
-          and sin_t.is_contiguous(), f"rotation tables are float32 [positions, {hd // 2}]")
+    if not (cos_t.shape == sin_t.shape and cos_t.shape[1] == hd // 2 and cos_t.dtype is sin_t.dtype is torch.float32 and cos_t.is_contiguous()
+            and sin_t.is_contiguous()):
+        raise ValueError(f"rotation tables are float32 [positions, {hd // 2}]")
 
 
 def acc_rope_cache8(acc, dtype, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV, hd):
@@ -140,21 +174,21 @@ def acc_rope_cache8(acc, dtype, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_sca
     bs = k8.shape[2]
     T, W = acc.shape
     _check_cache("acc_rope_cache8", k8, v8, k_scale, v_scale, H, KV, hd)
-    _check_slots("acc_rope_cache8", slots, bs, k8.shape[0])
-    _debug.check_range("acc_rope_cache8", "positions", pos, 0, cos_t.shape[0])
+    if _debug.ENABLED:
+        _check_slots("acc_rope_cache8", slots, bs, k8.shape[0])
+        _debug.check_range("acc_rope_cache8", "positions", pos, 0, cos_t.shape[0])
     _need(acc.dtype == torch.float32 and acc.is_contiguous() and W == (H + 2 * KV) * hd, "acc_rope_cache8: a float32 accumulator of whole rows")
-    _need(pos.shape == slots.shape == (T,) and pos.dtype == torch.int32 and slots.dtype == torch.int64 and pos.is_contiguous() and slots.is_contiguous(),
-          "acc_rope_cache8: a position (int32) and a slot (int64) for each row")
-    if not _lib.use_native(acc):
+    _check_places("acc_rope_cache8", pos, slots, T)
+    if not acc.is_cuda:
         out = rope_cache8_ref(acc.to(dtype), pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV, hd)
         acc.zero_()
         return out
-    _check_device("acc_rope_cache8", acc, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale)
+    dev = _check_device("acc_rope_cache8", acc, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale)
     _check_tables(cos_t, sin_t, hd)
     out = torch.empty((T, W), dtype=dtype, device=acc.device)
-    f = _lib.fn("dlti_acc_rope_cache8", [_V, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V])
+    f = _fn("dlti_acc_rope_cache8", (_V, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V))
     _lib.check(f(acc.data_ptr(), out.data_ptr(), W, pos.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), slots.data_ptr(), k8.data_ptr(), v8.data_ptr(),
-                 k_scale.data_ptr(), v_scale.data_ptr(), T, H, KV, hd, bs, _lib.dtype_code(dtype), _lib.stream_ptr()), "acc_rope_cache8")
+                 k_scale.data_ptr(), v_scale.data_ptr(), T, H, KV, hd, bs, _lib.dtype_code(dtype), _stream(dev)), "acc_rope_cache8")
     return out
 
 
@@ -175,8 +209,13 @@ def paged_decode8_ref(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV
 
 
 def splits8(ctas: int, reach: int) -> int:
-    """CTAs over which contexts of up to `reach` tokens are cut when one each would be `ctas`: one wave of three per SM, 64 tokens at least."""
-    return max(1, min(64, 3 * 148 // max(1, ctas), -(-reach // 64)))
+    """CTAs over which contexts of up to `reach` tokens are cut when one each would be `ctas`: one wave of three per SM (a second one costs what it
+    should save), 64 tokens at least. Up to 8 are one cluster, more are clusters of one size. us, 4 rows of 30011 tokens with 8 key heads: 6 splits
+    72, 8 59, 12 57, 16 (two waves) 70; 32 rows of 4000 tokens with 4 key heads: 1 split 49, 2 41, 3 37, 4 (two waves) 49."""
+    n = max(1, min(128, 3 * 148 // max(1, ctas), -(-reach // 64)))
+    while n % -(-n // 8):
+        n -= 1
+    return n
 
 
 def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd, scale=None, out=None, max_ctx: int | None = None):
@@ -184,27 +223,35 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
     0 = a row of zeros; max_ctx: the longest context that may occur (a context beyond it is read in full). Returns out [B, H hd]."""
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     _check_cache("paged_decode8", k8, v8, k_scale, v_scale, H, KV, hd)
-    B = q.shape[0]
-    _need(q.dim() == 2 and q.shape[1] >= H * hd, "paged_decode8: rows of at least H hd columns")
-    _need(block_tables.dtype == ctx_lens.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == B and ctx_lens.shape == (B,)
-          and block_tables.is_contiguous() and ctx_lens.is_contiguous(), "paged_decode8: an int32 table and an int32 length for each row")
-    _need(out is None or (out.shape == (B, H * hd) and out.dtype == q.dtype and out.stride(1) == 1), "paged_decode8: out is [B, H hd] in q's type")
-    _debug.check_paged("paged_decode8", block_tables, ctx_lens, k8.shape[0], k8.shape[2])
-    if not _lib.use_native(q):
+    B, W = q.shape
+    if W < H * hd:
+        raise ValueError("paged_decode8: rows of at least H hd columns")
+    if not (block_tables.dtype is torch.int32 and ctx_lens.dtype is torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == B
+            and ctx_lens.shape == (B,) and block_tables.is_contiguous() and ctx_lens.is_contiguous()):
+        raise ValueError("paged_decode8: an int32 table and an int32 length for each row")
+    if out is not None:
+        _need(out.shape == (B, H * hd) and out.dtype == q.dtype and out.stride(1) == 1, "paged_decode8: out is [B, H hd] in q's type")
+    if _debug.ENABLED:
+        _debug.check_paged("paged_decode8", block_tables, ctx_lens, k8.shape[0], k8.shape[2])
+    if not q.is_cuda:
         o = paged_decode8_ref(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd, scale)
         return o if out is None else out.copy_(o)
-    _check_device("paged_decode8", q, k8, v8, k_scale, v_scale, block_tables, ctx_lens)
-    _need(q.stride(1) == 1 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0, "paged_decode8: rows begin at multiples of 16 bytes")
-    bs, reach = k8.shape[2], block_tables.shape[1] * k8.shape[2]
+    dev = _check_device("paged_decode8", q, k8, v8, k_scale, v_scale, block_tables, ctx_lens)
+    ld, unit = q.stride()
+    if unit != 1 or ld % 8 or q.data_ptr() % 16:
+        raise ValueError("paged_decode8: rows begin at multiples of 16 bytes")
+    bs, width = k8.shape[2], block_tables.shape[1]
     if out is None:
         out = torch.empty((B, H * hd), dtype=q.dtype, device=q.device)
-    splits = splits8(B * KV * -(-(H // KV) // 8), reach if max_ctx is None else min(reach, max_ctx))
+    else:
+        _check_device("paged_decode8", out)
+    splits = splits8(B * KV * -(-(H // KV) // 8), width * bs if max_ctx is None else min(width * bs, max_ctx))
     # a workspace of this call's own: the allocator keeps it for the stream's later work, or inside the graph that captures it
-    ws = torch.empty(B * H * splits * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-    f = _lib.fn("dlti_paged_decode8", [_V, _L, _V, _V, _V, _V, _V, _I, _V, _I, _I, _I, _I, _I, _F, _I, _V, _V, _L, _I, _V])
-    _lib.check(f(q.data_ptr(), q.stride(0), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
-                 block_tables.shape[1], ctx_lens.data_ptr(), B, bs, H, KV, hd, float(scale), splits, None if ws is None else ws.data_ptr(),
-                 out.data_ptr(), out.stride(0), _lib.dtype_code(q.dtype), _lib.stream_ptr()), "paged_decode8")
+    ws = torch.empty(B * H * -(-splits // 8) * (hd + 2), dtype=torch.float32, device=q.device) if splits > 8 else None
+    f = _fn("dlti_paged_decode8", (_V, _L, _V, _V, _V, _V, _V, _I, _V, _I, _I, _I, _I, _I, _F, _I, _V, _V, _L, _I, _V))
+    _lib.check(f(q.data_ptr(), ld, k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+                 width, ctx_lens.data_ptr(), B, bs, H, KV, hd, scale, splits, None if ws is None else ws.data_ptr(),
+                 out.data_ptr(), out.stride(0), _lib.dtype_code(q.dtype), _stream(dev)), "paged_decode8")
     return out
 
 
@@ -221,15 +268,17 @@ def gather_rows8_(ext, rows, slots, k8, v8, k_scale, v_scale, H, KV, hd):
     """Key and value columns of the rows `rows` (int64 [n], each once) of ext [*, (H + 2 KV) hd] from the cached tokens at `slots` (int64 [n]), in
     ext's type. Returns ext; its other rows and columns stay as they are."""
     _check_cache("gather_rows8", k8, v8, k_scale, v_scale, H, KV, hd)
-    _need(rows.dim() == 1 and rows.shape == slots.shape and rows.dtype == slots.dtype == torch.int64 and rows.is_contiguous() and slots.is_contiguous(),
-          "gather_rows8: an int64 row for each int64 slot")
-    _debug.check_range("gather_rows8", "slots", slots, 0, k8.shape[0] * k8.shape[2])
-    _debug.check_range("gather_rows8", "rows", rows, 0, ext.shape[0])
-    if not _lib.use_native(ext):
+    if not (rows.dim() == 1 and rows.shape == slots.shape and rows.dtype is torch.int64 and slots.dtype is torch.int64 and rows.is_contiguous()
+            and slots.is_contiguous()):
+        raise ValueError("gather_rows8: an int64 row for each int64 slot")
+    if _debug.ENABLED:
+        _debug.check_range("gather_rows8", "slots", slots, 0, k8.shape[0] * k8.shape[2])
+        _debug.check_range("gather_rows8", "rows", rows, 0, ext.shape[0])
+    if not ext.is_cuda:
         return gather_rows8_ref(ext, rows, slots, k8, v8, k_scale, v_scale, H, KV, hd)
-    _check_device("gather_rows8", ext, rows, slots, k8, v8, k_scale, v_scale)
+    dev = _check_device("gather_rows8", ext, rows, slots, k8, v8, k_scale, v_scale)
     _check_rows("gather_rows8", ext, (H + 2 * KV) * hd)
-    f = _lib.fn("dlti_gather_rows8", [_V, _L, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V])
+    f = _fn("dlti_gather_rows8", (_V, _L, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V))
     _lib.check(f(ext.data_ptr(), ext.stride(0), rows.data_ptr(), slots.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
-                 v_scale.data_ptr(), slots.numel(), H, KV, hd, k8.shape[2], _lib.dtype_code(ext.dtype), _lib.stream_ptr()), "gather_rows8")
+                 v_scale.data_ptr(), slots.numel(), H, KV, hd, k8.shape[2], _lib.dtype_code(ext.dtype), _stream(dev)), "gather_rows8")
     return ext

@@ -2,48 +2,69 @@
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import torch
 
 from . import _lib
 
-_P = C.POINTER
+_TYPES = [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
 
 
-def check_copies(src: list[int], dst: list[int], num_pages: int) -> list[tuple[int, int]]:
-    """The pairs of a call, without those that copy a page onto itself. Refused: pages outside the cache, a page written twice, a page both read
-    and written (copies have no order)."""
+def check_copies(src: list[int], dst: list[int], num_pages: int) -> tuple[list[int], list[int]]:
+    """The sources and destinations of a call, without those that copy a page onto itself. Refused: pages outside the cache, a page written twice, a
+    page both read and written (copies have no order)."""
     if len(src) != len(dst):
         raise ValueError(f"copy_pages: {len(src)} sources for {len(dst)} destinations")
-    if any(not 0 <= p < num_pages for p in (*src, *dst)):
+    if not src:
+        return src, dst
+    if min(src) < 0 or min(dst) < 0 or max(src) >= num_pages or max(dst) >= num_pages:
         raise ValueError(f"copy_pages: pages are 0 .. {num_pages - 1}")
-    if len(set(dst)) < len(dst):
+    written = set(dst)
+    if len(written) < len(dst):
         raise ValueError("copy_pages: a page is written twice")
-    pairs = [(a, b) for a, b in zip(src, dst) if a != b]
-    if {a for a, _ in pairs} & {b for _, b in pairs}:
-        raise ValueError("copy_pages: a page is both read and written")
-    return pairs
+    if not written.isdisjoint(src):
+        pairs = [(a, b) for a, b in zip(src, dst) if a != b]
+        src, dst = [a for a, _ in pairs], [b for _, b in pairs]
+        if not set(dst).isdisjoint(src):
+            raise ValueError("copy_pages: a page is both read and written")
+    return src, dst
+
+
+def _page(t: torch.Tensor, page_dim: int) -> tuple[int, int, int, int]:
+    """(layers, bytes from layer to layer, bytes from page to page, bytes of a page) of a cache."""
+    shape, stride, es = t.shape, t.stride(), t.element_size()
+    n = 1
+    for d in range(len(shape) - 1, page_dim, -1):
+        if shape[d] != 1 and stride[d] != n:
+            raise ValueError("copy_pages: what a page holds is contiguous")
+        n *= shape[d]
+    if shape[page_dim] > 1 and stride[page_dim] < n:
+        raise ValueError("copy_pages: pages do not overlap")
+    return (shape[0], stride[0] * es, stride[1] * es, n * es) if page_dim else (1, 0, stride[0] * es, n * es)
 
 
 def copy_pages(caches: list[torch.Tensor], src: list[int], dst: list[int], page_dim: int = 0) -> None:
     """Pages src[i] -> dst[i] (whole numbers on the host) of every tensor in `caches`: [pages, ...], or with page_dim=1 [layers, pages, ...]. What a
-    page holds is contiguous. One launch for up to 32 tensors and 300 pairs."""
+    page holds is contiguous. One launch for up to 32 tensors and 300 pairs; the pairs travel with it, so a graph that captures the call replays
+    these."""
     if page_dim not in (0, 1):
         raise ValueError("copy_pages: pages are dimension 0, or dimension 1 behind the layers")
     if not caches:
         return
-    counts = {t.shape[page_dim] for t in caches}
-    if len(counts) > 1:
-        raise ValueError(f"copy_pages: caches of {sorted(counts)} pages")
-    pairs = check_copies(src, dst, counts.pop())
+    num = caches[0].shape[page_dim]
     for t in caches:
-        one = t.select(page_dim, 0)
-        if not (one if page_dim == 0 else one.select(0, 0)).is_contiguous():
-            raise ValueError("copy_pages: what a page holds is contiguous")
-    if not pairs:
+        if t.shape[page_dim] != num:
+            raise ValueError(f"copy_pages: caches of {num} and {t.shape[page_dim]} pages")
+    src, dst = check_copies(src, dst, num)
+    flat = []
+    for t in caches:
+        flat.append(t.data_ptr())
+        flat += _page(t, page_dim)
+    if not src:
         return
-    if not _lib.use_native(*caches):
-        a, b = (torch.tensor(p) for p in zip(*pairs))
+    if not caches[0].is_cuda:
+        a, b = torch.tensor(src), torch.tensor(dst)
         for t in caches:
             if page_dim == 0:
                 t[b] = t[a]
@@ -51,17 +72,10 @@ def copy_pages(caches: list[torch.Tensor], src: list[int], dst: list[int], page_
                 t[:, b] = t[:, a]
         return
     d = torch.cuda.current_device()
-    if any(not t.is_cuda or t.device.index != d for t in caches):
-        raise ValueError(f"copy_pages: every cache is on the current device, cuda:{d}")
-    n = len(caches)
-    es = [t.element_size() for t in caches]
-    layers = [t.shape[0] if page_dim else 1 for t in caches]
-    page = [t.stride(page_dim) * e for t, e in zip(caches, es)]
-    layer = [t.stride(0) * e if page_dim else 0 for t, e in zip(caches, es)]
-    size = [t[(0,) * (page_dim + 1)].numel() * e for t, e in zip(caches, es)]
-    f = _lib.fn("dlti_copy_pages", [C.c_void_p, _P(C.c_int), _P(C.c_longlong), _P(C.c_longlong), _P(C.c_longlong), C.c_int, _P(C.c_int), _P(C.c_int),
-                                    C.c_int, C.c_void_p])
-    m = len(pairs)
-    _lib.check(f((C.c_void_p * n)(*[t.data_ptr() for t in caches]), (C.c_int * n)(*layers), (C.c_longlong * n)(*layer), (C.c_longlong * n)(*page),
-                 (C.c_longlong * n)(*size), n, (C.c_int * m)(*[p[0] for p in pairs]), (C.c_int * m)(*[p[1] for p in pairs]), m, _lib.stream_ptr()),
+    for t in caches:
+        if t.get_device() != d:
+            raise ValueError(f"copy_pages: every cache is on the current device, cuda:{d}")
+    f = _lib.fn("dlti_copy_pages", _TYPES)
+    what, a, b = array("q", flat), array("i", src), array("i", dst)
+    _lib.check(f(what.buffer_info()[0], len(caches), a.buffer_info()[0], b.buffer_info()[0], len(a), torch._C._cuda_getCurrentRawStream(d)),
                "copy_pages")

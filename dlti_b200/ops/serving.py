@@ -270,28 +270,34 @@ def sample_given(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
     which the running sum of what is kept exceeds u times its sum. Temperature <= 0: the largest logit at its lowest index. NaN counts as -inf; a
     row of nothing else gives token 0 and log-prob -inf. The same logits and numbers give the same tokens everywhere."""
     B, V = logits.shape
-    if u.dtype != torch.float64 or u.shape != (B,) or not u.is_contiguous():
+    if u.dtype is not torch.float64 or u.shape != (B,) or not u.is_contiguous():
         raise ValueError("sample_given: a float64 number for each row")
-    for name, t, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                        ("min_p", min_p, torch.float32)):
-        if t is not None and (t.dtype != dt or t.shape != (B,) or not t.is_contiguous()):
+    for t, name, dt in ((temperature, "temperature", torch.float32), (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                        (min_p, "min_p", torch.float32)):
+        if t is not None and (t.dtype is not dt or t.shape != (B,) or not t.is_contiguous()):
             raise ValueError(f"sample_given: {name} is {dt} [{B}]")
-    if out is not None and (out.dtype != torch.int64 or out.shape != (B,) or not out.is_contiguous()):
+    if out is not None and (out.dtype is not torch.int64 or out.shape != (B,) or not out.is_contiguous()):
         raise ValueError(f"sample_given: out is int64 [{B}]")
     if not 1 <= V <= 1 << 18:
         raise ValueError(f"sample_given: rows of 1 to 262144 logits, got {V}")
-    if not _lib.use_native(logits):
+    if not logits.is_cuda:
         tok, lp = sample_given_ref(logits, u, temperature, top_k, top_p, min_p)
         return tok if out is None else out.copy_(tok), lp if want_logprob else None
-    if logits.stride(1) != 1:
+    ld, unit = logits.stride()
+    if unit != 1:
         raise ValueError("sample_given: a row's logits are consecutive")
     d = torch.cuda.current_device()
-    if any(t is not None and (not t.is_cuda or t.device.index != d) for t in (logits, u, temperature, top_k, top_p, min_p, out)):
-        raise ValueError(f"sample_given: every tensor is on the current device, cuda:{d}")
+    for t in (logits, u, temperature, top_k, top_p, min_p, out):
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"sample_given: every tensor is on the current device, cuda:{d}")
     if out is None:
         out = torch.empty(B, dtype=torch.int64, device=logits.device)
     lp = torch.empty(B, dtype=torch.float32, device=logits.device) if want_logprob else None
-    f = _lib.fn("dlti_sample_given", [_V, _L, _I, _I, _V, _V, _V, _V, _V, _V, _V, _I, _V])
-    _lib.check(f(_lib.ptr(logits), logits.stride(0), B, V, _lib.ptr(u), _lib.ptr(temperature), _lib.ptr(top_k), _lib.ptr(top_p), _lib.ptr(min_p),
-                 _lib.ptr(out), _lib.ptr(lp), _lib.dtype_code(logits.dtype), _lib.stream_ptr()), "sample_given")
+    f = _lib.fn("dlti_sample_given", _GIVEN)
+    p = [None if t is None else t.data_ptr() for t in (temperature, top_k, top_p, min_p, lp)]
+    _lib.check(f(logits.data_ptr(), ld, B, V, u.data_ptr(), p[0], p[1], p[2], p[3], out.data_ptr(), p[4], _lib.dtype_code(logits.dtype),
+                 torch._C._cuda_getCurrentRawStream(d)), "sample_given")
     return out, lp
+
+
+_GIVEN = [_V, _L, _I, _I, _V, _V, _V, _V, _V, _V, _V, _I, _V]

@@ -365,7 +365,7 @@ int dlti_rope_cache8(const void* x, long long x_ld, void* out, long long out_ld,
 int dlti_acc_rope_cache8(float* acc, void* out, long long out_ld, const int* pos, const float* cos_t, const float* sin_t,
                          const long long* slots, void* k8, void* v8, float* ks, float* vs, long long tokens, int H, int KV, int hd, int bs,
                          int dtype, dlti_stream_t stream);
-/* attention of single tokens; workspace: dlti_paged_decode8_floats, none for one split */
+/* attention of single tokens; splits 1 .. 128, the same number in each of ceil(splits / 8) clusters; workspace: dlti_paged_decode8_floats, none for up to 8 */
 long long dlti_paged_decode8_floats(int batch, int H, int splits);
 int dlti_paged_decode8(const void* q, long long q_ld, const void* k8, const void* v8, const float* ks, const float* vs, const int* tables,
                        int max_blocks, const int* ctx, int batch, int bs, int H, int KV, int hd, float scale, int splits, float* workspace,
@@ -373,9 +373,9 @@ int dlti_paged_decode8(const void* q, long long q_ld, const void* k8, const void
 /* key and value columns of ext's rows rows[0..n) from the cached tokens at slots[0..n) */
 int dlti_gather_rows8(void* ext, long long ext_ld, const long long* rows, const long long* slots, const void* k8, const void* v8, const float* ks,
                       const float* vs, long long n, int H, int KV, int hd, int bs, int dtype, dlti_stream_t stream);
-/* pages from[i] -> to[i] (host arrays) of every layer of every cache: csrc/pages.cu */
-int dlti_copy_pages(void* const* bases, const int* layers, const long long* layer_bytes, const long long* page_stride, const long long* page_bytes,
-                    int caches, const int* from, const int* to, int pairs, dlti_stream_t stream);
+/* pages from[i] -> to[i] of every layer of every cache (host arrays): caches[5 c ...] = base address, layers, bytes from layer to layer, bytes
+ * from page to page, bytes of a page. csrc/pages.cu */
+int dlti_copy_pages(const long long* caches, int count, const int* from, const int* to, int pairs, dlti_stream_t stream);
 /* out[t] = src[t] in [0, n) ? sampled[src[t]] : ids[t]: the input ids of a step that continues the step in flight */
 int dlti_feed_ids(const long long* ids, const int* src, const long long* sampled, int n, long long* out, long long rows,
                   dlti_stream_t stream);

@@ -225,6 +225,13 @@ def test_attend(dev, dtype, lens, H, KV, bs):
     check_attend(lens, H, KV, bs, dtype, dev, seed=len(lens) + H)
 
 
+def test_splits_are_clusters_of_one_size():
+    for ctas in (*range(1, 500), 5000):
+        for reach in (1, 64, 65, 600, 5000, 100000):
+            n = kv8.splits8(ctas, reach)
+            assert 1 <= n <= 128 and n % -(-n // 8) == 0 and n <= max(1, -(-reach // 64)) and (n == 1 or n * ctas <= 444)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("max_ctx", [None, 100, 4096])
 def test_attend_reach(dev, max_ctx):

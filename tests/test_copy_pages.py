@@ -60,7 +60,7 @@ def test_refusals():
     for src, dst in (([0], [8]), ([-1], [2]), ([0, 1], [2]), ([0, 1], [2, 2]), ([0, 2], [2, 3]), ([0, 1], [1, 0])):
         with pytest.raises(ValueError):
             copy_pages([a], src, dst, page_dim=1)
-    for caches, dim in (([a, torch.zeros(3, 9, 4)], 1), ([a], 2), ([a.transpose(0, 2)], 1)):
+    for caches, dim in (([a, torch.zeros(3, 9, 4)], 1), ([a], 2), ([a.transpose(0, 2)], 1), ([a[:, :1].expand(3, 8, 4)], 1)):
         with pytest.raises(ValueError):
             copy_pages(caches, [0], [1], page_dim=dim)
-    assert check_copies([1, 2, 2], [1, 3, 4], 5) == [(2, 3), (2, 4)]
+    assert check_copies([1, 2, 2], [1, 3, 4], 5) == ([2, 2], [3, 4])
