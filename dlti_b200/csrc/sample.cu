@@ -6,12 +6,15 @@
 // on the order of atomics, and with up to 2^18 of them stay below 2^63.
 //
 // The kept tokens are a prefix of the order (logit descending, index ascending); each cut is found as the last token that it keeps, a 64-bit
-// number of the logit's order-preserving bits and the index. A CTA takes a row and reads it several times, after the first time from L2:
-//   1. the largest logit and the sum for the log-probability,
-//   2. counts over 2048 bins of the logit's distance from the largest: the bin in which top-k ends, and bounds for the bin in which top-p ends,
-//   3. the exact sums: of everything, above those bins, and of each of them; then the few tokens of the one bin are ranked by themselves,
-//   4. the kept weights of every 256 tokens; of these the group, the lane and the token that the given number falls on.
-// A bin of too many tokens (equal logits, or logits in a narrow range) is divided further by 11 bits of the logit at a time.
+// number of the logit's order-preserving bits and the index. A CTA takes a row and reads it three times, after the first time from L2:
+//   1. the largest logit,
+//   2. the sum for the log-probability, and counts over 8192 bins of the distance from the largest: the bin in which top-k ends, and bounds for
+//      the bins in which top-p can end,
+//   3. the weights: tokens before these bins are kept whatever comes and go into sums of 256 tokens each; the tokens of these bins, some
+//      thousand of a whole vocabulary, go to a list with their weights.
+// The list then says where the cuts lie and is added to the sums; of these the group, the lane and the token follow that the number falls on.
+// Where the list does not hold those bins' tokens (equal logits, or logits in a narrow range) a bin is divided further by 11 bits of the logit at a
+// time, and the row read once more for each division, once for the ranks and once for the sums.
 #include "common.cuh"
 
 namespace {
@@ -20,15 +23,24 @@ typedef unsigned long long u64;
 
 constexpr int TH = 1024, PER = 8;                 // threads, and consecutive tokens of a thread in a chunk
 constexpr int CHUNK = TH * PER;
-constexpr int NB = 2 * TH, LIST = 1024;
+constexpr int NB = 8 * TH, ND = 2 * TH;            // bins of the distance from the largest; digits of 11 bits
+constexpr int LIST = 512, WINDOW = 7168;
 constexpr int V_MAX = 1 << 18;
 constexpr double UNIT = 35184372088832.0;         // 2^45
 constexpr float RANGE = 32.f;                     // bins reach this far below the largest logit, in units of T: e^-32 < 2^-46
 
 struct Work {
-  uint32_t cnt[NB];
-  u64 mass[NB];
-  u64 lc[LIST], lw[LIST];
+  uint32_t bins[NB];                              // tokens of each bin
+  uint32_t cnt[ND];
+  u64 mass[ND];
+  union {
+    struct {
+      u64 lc[LIST], lw[LIST];                     // tokens of one bin, and their weights
+    };
+    struct {
+      u64 wc[WINDOW], ww[WINDOW];                 // tokens of all bins in which a cut may lie
+    };
+  };
   u64 cw[V_MAX / (32 * PER)];
   u64 red[32];
   float fred[32];
@@ -42,12 +54,22 @@ struct Row {
   const T* p;
   int V;
   bool vec;
+  struct Raw {
+    int4 v[sizeof(T) / 2];
+  };
+  __device__ __forceinline__ Raw fetch(int base) const {
+    Raw r;
+    if (vec && base + PER <= V) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = reinterpret_cast<const int4*>(p + base)[i];
+    }
+    return r;
+  }
   // tokens base .. base + 7; those behind the end and NaN as -inf
-  __device__ __forceinline__ void get(int base, float (&x)[PER]) const {
+  __device__ __forceinline__ void open(const Raw& r, int base, float (&x)[PER]) const {
     if (vec && base + PER <= V) {
       if constexpr (sizeof(T) == 2) {
-        const int4 v = *reinterpret_cast<const int4*>(p + base);
-        const uint32_t u[4] = {(uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w};
+        const uint32_t u[4] = {(uint32_t)r.v[0].x, (uint32_t)r.v[0].y, (uint32_t)r.v[0].z, (uint32_t)r.v[0].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float2 f = Cvt<T>::unpack2(u[i]);
@@ -55,29 +77,89 @@ struct Row {
           x[2 * i + 1] = f.y;
         }
       } else {
-        const float4 a = *reinterpret_cast<const float4*>(p + base), b = *reinterpret_cast<const float4*>(p + base + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x[4 * i] = __int_as_float(r.v[i].x);
+          x[4 * i + 1] = __int_as_float(r.v[i].y);
+          x[4 * i + 2] = __int_as_float(r.v[i].z);
+          x[4 * i + 3] = __int_as_float(r.v[i].w);
+        }
       }
     } else {
 #pragma unroll
       for (int j = 0; j < PER; ++j) x[j] = base + j < V ? Cvt<T>::to_f(p[base + j]) : -INFINITY;
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) x[j] = x[j] != x[j] ? -INFINITY : x[j] + 0.f;      // -0 is 0
+    for (int j = 0; j < PER; ++j) x[j] = fmaxf(x[j], -INFINITY);                     // NaN is -inf
+  }
+  __device__ __forceinline__ void get(int base, float (&x)[PER]) const { open(fetch(base), base, x); }
+  // body(chunk, base, tokens) for all of the thread's tokens; two chunks are on their way meanwhile
+  template <typename F>
+  __device__ __forceinline__ void each_chunk(F&& body) const {
+    const int chunks = (V + CHUNK - 1) / CHUNK;
+    int base = threadIdx.x * PER;
+    Raw a = fetch(base), n = fetch(base + CHUNK);
+    for (int c = 0; c < chunks; ++c, base += CHUNK) {
+      const Raw m = fetch(base + 2 * CHUNK);
+      float x[PER];
+      open(a, base, x);
+      body(c, base, x);
+      a = n;
+      n = m;
+    }
   }
 };
 
 __device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);                         // -0 is 0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ u64 place(float x, int i) { return (u64)key_of(x) << 32 | (0xffffffffu - (uint32_t)i); }
-__device__ __forceinline__ float below(float top, float x) { return x == top ? 0.f : top - x; }
-__device__ __forceinline__ int bin_of(float d, float per_bin) { return (int)fminf(d * per_bin, (float)(NB - 1)); }
-__device__ __forceinline__ u64 weight(float top, float x, double inv_t) {
-  if (x == top) return (u64)UNIT;
-  return x == -INFINITY || top == INFINITY ? 0 : __double2ull_rn(exp(((double)x - (double)top) * inv_t) * UNIT);
+__device__ __forceinline__ float below(float top, float x) { return fmaxf(top - x, 0.f); }      // inf - inf is nothing
+__device__ __forceinline__ float logit_of(u64 c) {
+  const uint32_t k = (uint32_t)(c >> 32);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+__device__ __forceinline__ int bin_of(float d, float per_bin) { return (int)fminf(d * per_bin, (float)(NB - 1)); }
+// A token's weight 2^(-(top - x) c), c = log2(e) / T, in units of 2^-45. 2^r on [-1/2, 1/2] is the polynomial of degree 9 through its values at the
+// Chebyshev nodes: relatively 2^-45.6 off at most, and 2^45 of the largest logit's own. 15 operations in double precision, at half the rate of
+// those in single, which is why a row's weights are taken once.
+__constant__ double POLY[12] = {0x1.000000000003dp+0, 0x1.62e42fefa39f7p-1, 0x1.ebfbdff8149f2p-3, 0x1.c6b08d7044119p-5, 0x1.3b2ab72b175eep-7,
+                                0x1.5d87fe908f88ap-10, 0x1.43088e257f341p-13, 0x1.ffcb76789860fp-17, 0x1.63ef969a64d3cp-20,
+                                0x1.b6571de2f2351p-24, 6755399441055744.0, 4503599627370496.0};
+constexpr float NOTHING = 47.f * NB / (RANGE * 1.4426950408889634f);   // in bins: weights below 2^-47
+struct Weigh {
+  float top, per_bin;
+  double top64, c;
+  __device__ __forceinline__ Weigh(float top_, float t)
+      : top(top_), per_bin((float)NB / (RANGE * t)), top64(wide(top_)), c(1.4426950408889634074 / (double)t) {}
+  // x in double by its bits (a conversion runs at a quarter of the rate): numbers below 2^-126 become others of that size, infinity 2^128
+  static __device__ __forceinline__ double wide(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return __hiloint2double((int)(((u & 0x7fffffffu) >> 3) + 0x38000000u | (u & 0x80000000u)), (int)(u << 29));
+  }
+  __device__ __forceinline__ u64 operator()(float x) const { return (*this)(x, below(top, x) * per_bin); }
+  // at: the distance in bins
+  __device__ __forceinline__ u64 operator()(float x, float at) const {
+    const double z = (top64 - wide(x)) * c;
+    const double y = z + POLY[10];                 // 1.5 * 2^52: the sum's low bits are the nearest whole number
+    const double r = (y - POLY[10]) - z;
+    double p = POLY[9];
+#pragma unroll
+    for (int i = 8; i >= 0; --i) p = fma(p, r, POLY[i]);
+    p = __hiloint2double(__double2hiint(p) + ((45 - __double2loint(y)) << 20), __double2loint(p));
+    const u64 w = (u64)__double_as_longlong(p + POLY[11]) & 0xfffffffffffffull;
+    return at <= NOTHING ? w : 0;                  // nothing, too, where the distance is no number
+  }
+};
+
+// A run of 2^shift bins among those that follow bin `base`.
+struct Group {
+  float top, per_bin;
+  int base, shift, g;
+  __device__ __forceinline__ int of(float x) const { return (bin_of(below(top, x), per_bin) - base) >> shift; }
+  __device__ __forceinline__ bool has(float x) const { return of(x) == g; }
+};
 
 template <typename S>
 __device__ __forceinline__ S warp_scan(S v) {                            // inclusive
@@ -107,9 +189,36 @@ __device__ __forceinline__ u64 cta_sum(u64 v, u64* red) {
   return total;
 }
 
-// The last token kept of a bin's tokens at or above `floor`: the r-th in order (MASS false), or the first at which the weights reach `want`.
+// Which of the counted digits (s.cnt, s.mass; s.i0 = -1) the cut lies in: the last one that is there, if sums fall short of it. What lies before it is
+// taken from r or `want`.
+template <bool MASS>
+__device__ __forceinline__ int digit(Work& s, uint32_t& r, double& want) {
+  const int tid = threadIdx.x;
+  const uint32_t c0 = s.cnt[2 * tid], c1 = s.cnt[2 * tid + 1];
+  const u64 v0 = MASS ? s.mass[2 * tid] : c0, v1 = MASS ? s.mass[2 * tid + 1] : c1;
+  u64 all;
+  const u64 after = cta_scan<u64>(v0 + v1, s.red, all);
+  const u64 b0 = after - v0 - v1, b1 = after - v1;
+  const double capped = fmin(MASS ? want : (double)r, (double)all);
+  if (c0 && (double)b0 < capped && capped <= (double)b1) { s.i0 = 2 * tid; s.u0 = b0; }
+  if (c1 && (double)b1 < capped && capped <= (double)after) { s.i0 = 2 * tid + 1; s.u0 = b1; }
+  __syncthreads();
+  const bool none = s.i0 < 0;
+  __syncthreads();
+  if (none) {                                                          // no weight at all: everything is kept up to the last token there is
+    if (c0) atomicMax(&s.i0, 2 * tid);
+    if (c1) atomicMax(&s.i0, 2 * tid + 1);
+    if (tid == 0) s.u0 = all;
+    __syncthreads();
+  }
+  if (MASS) want -= (double)s.u0;
+  else r -= (uint32_t)s.u0;
+  return s.i0;
+}
+
+// The last token kept of a group's n tokens at or above `floor`: the r-th in order (MASS false), or the first at which the weights reach `want`.
 template <bool MASS, typename T>
-__device__ u64 last_kept(const Row<T>& row, Work& s, float top, float per_bin, double inv_t, int bin, u64 floor, uint32_t n, uint32_t r, double want) {
+__device__ __noinline__ u64 last_kept(const Row<T> row, Work& s, const Weigh weigh, const Group group, u64 floor, uint32_t n, uint32_t r, double want) {
   const int tid = threadIdx.x;
   const int chunks = (row.V + CHUNK - 1) / CHUNK;
   int shift = 32;
@@ -121,7 +230,7 @@ __device__ u64 last_kept(const Row<T>& row, Work& s, float top, float per_bin, d
       row.get(base, x);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const bool in = base + j < row.V && bin_of(below(top, x[j]), per_bin) == bin && place(x[j], base + j) >= floor &&
+        const bool in = base + j < row.V && group.has(x[j]) && place(x[j], base + j) >= floor &&
                         (shift == 32 || key_of(x[j]) >> shift == prefix);
         body(c, base + j, x[j], in);
       }
@@ -130,7 +239,7 @@ __device__ u64 last_kept(const Row<T>& row, Work& s, float top, float per_bin, d
   while (n > LIST && shift > 0) {
     const int wide = min(11, shift), low = shift - wide;
     const uint32_t mask = (1u << wide) - 1;
-    for (int i = tid; i < NB; i += TH) {
+    for (int i = tid; i < ND; i += TH) {
       s.cnt[i] = 0;
       s.mass[i] = 0;
     }
@@ -139,34 +248,13 @@ __device__ u64 last_kept(const Row<T>& row, Work& s, float top, float per_bin, d
       if (in) {
         const uint32_t d = mask - (key_of(x) >> low & mask);
         atomicAdd(&s.cnt[d], 1u);
-        if (MASS) atomicAdd(&s.mass[d], weight(top, x, inv_t));
+        if (MASS) atomicAdd(&s.mass[d], weigh(x));
       }
     });
     if (tid == 0) s.i0 = -1;
     __syncthreads();
-    // the digit in which the cut lies: the last one that is there, if sums fall short of it
-    const uint32_t c0 = s.cnt[2 * tid], c1 = s.cnt[2 * tid + 1];
-    const u64 v0 = MASS ? s.mass[2 * tid] : c0, v1 = MASS ? s.mass[2 * tid + 1] : c1;
-    u64 all;
-    const u64 after = cta_scan<u64>(v0 + v1, s.red, all);
-    const u64 b0 = after - v0 - v1, b1 = after - v1;
-    const double goal = MASS ? want : (double)r;
-    const double capped = fmin(goal, (double)all);
-    if (c0 && (double)b0 < capped && capped <= (double)b1) { s.i0 = 2 * tid; s.u0 = b0; }
-    if (c1 && (double)b1 < capped && capped <= (double)after) { s.i0 = 2 * tid + 1; s.u0 = b1; }
-    __syncthreads();
-    const bool none = s.i0 < 0;
-    __syncthreads();
-    if (none) {                                                        // no weight at all: everything is kept up to the last token there is
-      if (c0) atomicMax(&s.i0, 2 * tid);
-      if (c1) atomicMax(&s.i0, 2 * tid + 1);
-      if (tid == 0) s.u0 = all;
-      __syncthreads();
-    }
-    const int at = s.i0;
+    const int at = digit<MASS>(s, r, want);
     n = s.cnt[at];
-    if (MASS) want -= (double)s.u0;
-    else r -= (uint32_t)s.u0;
     prefix = prefix << wide | (mask - (uint32_t)at);
     shift = low;
     __syncthreads();
@@ -183,7 +271,7 @@ __device__ u64 last_kept(const Row<T>& row, Work& s, float top, float per_bin, d
         const uint32_t k = atomicAdd(&s.n, 1u);
         if (k < LIST) {
           s.lc[k] = place(x, i);
-          s.lw[k] = MASS ? weight(top, x, inv_t) : 1;
+          s.lw[k] = MASS ? weigh(x) : 1;
         }
       }
     });
@@ -207,9 +295,7 @@ __device__ u64 last_kept(const Row<T>& row, Work& s, float top, float per_bin, d
   }
   // many tokens with one logit: the r-th by index
   if (MASS) {
-    const uint32_t key = prefix;
-    const float x = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-    const double w = (double)weight(top, x, inv_t);
+    const double w = (double)weigh(logit_of((u64)prefix << 32));
     r = w > 0 ? (uint32_t)fmin(fmax(ceil(want / w), 1.0), (double)n) : n;
   }
   r = min(max(r, 1u), n);
@@ -254,6 +340,170 @@ __device__ u64 last_kept(const Row<T>& row, Work& s, float top, float per_bin, d
   return got;
 }
 
+// The same among those of the list's n tokens (s.wc).
+template <bool MASS>
+__device__ __noinline__ u64 ranked(Work& s, uint32_t n, const Group group, u64 floor, uint32_t r, double want) {
+  const int tid = threadIdx.x;
+  int shift = 64;
+  u64 prefix = 0;
+  auto in = [&](u64 c) { return c >= floor && group.has(logit_of(c)) && (shift == 64 || c >> shift == prefix); };
+  // their numbers in the list, in place of the counts
+  auto gather = [&]() {
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += TH)
+      if (in(s.wc[i])) {
+        const uint32_t k = atomicAdd(&s.n, 1u);
+        if (k < ND) s.cnt[k] = i;
+      }
+    __syncthreads();
+    const uint32_t m = s.n;
+    __syncthreads();
+    return m;
+  };
+  uint32_t m = gather();
+  while (m > LIST && shift > 0) {                                      // too many to compare each with each: 11 more bits
+    const int wide = min(11, shift), low = shift - wide;
+    const uint32_t mask = (1u << wide) - 1;
+    for (int i = tid; i < ND; i += TH) {
+      s.cnt[i] = 0;
+      s.mass[i] = 0;
+    }
+    if (tid == 0) s.i0 = -1;
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += TH) {
+      const u64 c = s.wc[i];
+      if (in(c)) {
+        const uint32_t d = mask - ((uint32_t)(c >> low) & mask);
+        atomicAdd(&s.cnt[d], 1u);
+        if (MASS) atomicAdd(&s.mass[d], s.ww[i]);
+      }
+    }
+    __syncthreads();
+    const int at = digit<MASS>(s, r, want);
+    prefix = prefix << wide | (mask - (uint32_t)at);
+    shift = low;
+    m = gather();
+  }
+  if (tid == 0) s.u0 = s.u1 = ~0ull;
+  __syncthreads();
+  for (uint32_t i = tid; i < m; i += TH) {
+    const u64 mine = s.wc[s.cnt[i]];
+    u64 before = 0;
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < m; ++j) {
+      const uint32_t e = s.cnt[j];
+      if (s.wc[e] > mine) {
+        before += s.ww[e];
+        ++rank;
+      }
+    }
+    if (MASS ? (double)before < want && want <= (double)(before + s.ww[s.cnt[i]]) : rank == r - 1) s.u0 = mine;
+    if (rank == m - 1) s.u1 = mine;                                    // sums that fall short of `want` keep all
+  }
+  __syncthreads();
+  const u64 got = s.u0 != ~0ull ? s.u0 : s.u1;
+  __syncthreads();
+  return got;
+}
+
+// Where top-p ends: the group in which the weights (s.mass, by group) reach `goal`, -1 if they do not; what is left of goal there.
+__device__ __forceinline__ int reached(Work& s, double& goal) {
+  const int tid = threadIdx.x;
+  const u64 m0 = s.mass[2 * tid], m1 = s.mass[2 * tid + 1];
+  u64 all;
+  const u64 after = cta_scan<u64>(m0 + m1, s.red, all);
+  const u64 b0 = after - m0 - m1, b1 = after - m1;
+  if (tid == 0) s.i0 = -1;
+  __syncthreads();
+  if (m0 && (double)b0 < goal && goal <= (double)b1) { s.i0 = 2 * tid; s.u0 = b0; }
+  if (m1 && (double)b1 < goal && goal <= (double)after) { s.i0 = 2 * tid + 1; s.u0 = b1; }
+  __syncthreads();
+  const int g = s.i0;
+  if (g >= 0) goal -= (double)s.u0;
+  __syncthreads();
+  return g;
+}
+
+// Both cuts where the list is too short. by_k: the bin in which top-k ends; by_p: the bins in which top-p can, from its base to `to`.
+template <typename T>
+__device__ __noinline__ u64 cut_by_division(const Row<T> row, Work& s, const Weigh weigh, bool k_on, Group by_k, uint32_t k_left, bool p_on, Group by_p, int to,
+                                            float tp) {
+  const int tid = threadIdx.x, V = row.V;
+  const int chunks = (V + CHUNK - 1) / CHUNK;
+  u64 floor = 0;
+  if (k_on) floor = last_kept<false>(row, s, weigh, by_k, 0ull, s.bins[by_k.g], k_left, 0.0);
+  if (!p_on) return floor;
+  for (int i = tid; i < ND; i += TH) {
+    s.cnt[i] = 0;
+    s.mass[i] = 0;
+  }
+  __syncthreads();
+  u64 whole = 0, above = 0;
+  const int groups = ((to - by_p.base) >> by_p.shift) + 1;
+  for (int c = 0; c < chunks; ++c) {
+    const int base = c * CHUNK + tid * PER;
+    float x[PER];
+    row.get(base, x);
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (base + j < V && place(x[j], base + j) >= floor) {
+        const u64 w = weigh(x[j]);
+        const int g = by_p.of(x[j]);
+        whole += w;
+        if (g < 0) above += w;
+        else if (g < groups) {
+          atomicAdd(&s.mass[g], w);
+          atomicAdd(&s.cnt[g], 1u);
+        }
+      }
+  }
+  whole = cta_sum(whole, s.red);
+  above = cta_sum(above, s.red);
+  double want = fmax((double)tp * (double)whole, 0.5) - (double)above;
+  by_p.g = reached(s, want);
+  if (by_p.g < 0) return floor;                                        // nothing is cut
+  const uint32_t n = s.cnt[by_p.g];
+  __syncthreads();
+  return last_kept<true>(row, s, weigh, by_p, floor, n, 0u, want);
+}
+
+// The weights of a row: sums of the tokens before bin f_first, by 256 tokens (of at least `least`) and altogether, and of all; the tokens of the bins
+// from there to f_last go to the list. EVERY: top-k is off, every token's weight counts. SUM: for top-p's sum. CUT: min-p is on.
+template <bool EVERY, bool SUM, bool CUT, typename T>
+__device__ __noinline__ void weights(const Row<T> row, Work& s, const Weigh weigh, float f_first, float f_last, u64 least, u64& whole_, u64& sure_) {
+  u64 whole = 0, sure = 0;
+  row.each_chunk([&](int c, int base, const float (&x)[PER]) {
+    u64 kept = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {                                    // those behind the end are -inf: no weight
+      const float at = below(weigh.top, x[j]) * weigh.per_bin;
+      if (EVERY || __any_sync(0xffffffffu, at < f_last)) {
+        const u64 w = EVERY || at < f_last ? weigh(x[j], at) : 0;
+        const u64 before = at < f_first ? w : 0;
+        if (SUM) whole += w;
+        if (CUT) {
+          sure += before;
+          kept += before >= least ? before : 0;
+        } else {
+          kept += before;
+        }
+        if (at >= f_first && at < f_last && base + j < row.V) {
+          const uint32_t i = atomicAdd(&s.n, 1u);
+          s.wc[i] = place(x[j], base + j);
+          s.ww[i] = w;
+        }
+      }
+    }
+    if (!CUT) sure += kept;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
+    if ((threadIdx.x & 31) == 0) s.cw[c * 32 + (threadIdx.x >> 5)] = kept;
+  });
+  whole_ = whole;
+  sure_ = sure;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict__ logits, long long ld, int V, const double* __restrict__ u,
                                                              const float* __restrict__ temperature, const int* __restrict__ top_k,
@@ -267,15 +517,17 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
   const int chunks = (V + CHUNK - 1) / CHUNK;
 
   // the largest logit, at its lowest index
-  u64 best = 0;
-  for (int c = 0; c < chunks; ++c) {
-    const int base = c * CHUNK + tid * PER;
-    float x[PER];
-    row.get(base, x);
+  float mine_top = -INFINITY;
+  int mine_at = tid * PER;
+  row.each_chunk([&](int, int base, const float (&x)[PER]) {
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (base + j < V) best = max(best, place(x[j], base + j));
-  }
+      if (x[j] > mine_top) {
+        mine_top = x[j];
+        mine_at = base + j;
+      }
+  });
+  u64 best = place(mine_top, mine_at);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (lane == 0) s.red[warp] = best;
@@ -284,8 +536,7 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   const int arg = (int)(0xffffffffu - (uint32_t)best);
-  const uint32_t bk = (uint32_t)(best >> 32);
-  const float top = __uint_as_float(bk & 0x80000000u ? bk & 0x7fffffffu : ~bk);
+  const float top = logit_of(best);
   __syncthreads();
   if (top == -INFINITY) {                                              // nothing is left: no token is more likely than another
     if (tid == 0) {
@@ -301,30 +552,26 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
   const float tp = drawn && top_p ? top_p[b] : 1.f;
   const bool p_on = tp < 1.f;
   const float tt = fmaxf(t, 1e-30f);                                   // the distances of a row in units of T stay finite
-  const double inv_t = drawn ? 1.0 / (double)tt : 1.0;
-  const float per_bin = (float)NB / (RANGE * tt);
+  const Weigh weigh(top, drawn ? tt : 1.f);
+  const float per_bin = weigh.per_bin;
 
-  if (drawn && (k_on || p_on)) {
-    for (int i = tid; i < NB; i += TH) {
-      s.cnt[i] = 0;
-      s.mass[i] = 0;
-    }
+  if (k_on || p_on) {
+    for (int i = tid; i < NB; i += TH) s.bins[i] = 0;
     __syncthreads();
   }
   float sum1 = 0.f;
-  if (out_logprob || (drawn && (k_on || p_on)))
-    for (int c = 0; c < chunks; ++c) {
-      const int base = c * CHUNK + tid * PER;
-      float x[PER];
-      row.get(base, x);
+  if (out_logprob || k_on || p_on)
+    row.each_chunk([&](int, int base, const float (&x)[PER]) {
+      if (out_logprob) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (base + j < V) {
-          const float d = below(top, x[j]);
-          if (out_logprob) sum1 += expf(-d);
-          if (k_on || p_on) atomicAdd(&s.cnt[bin_of(d, per_bin)], 1u);
-        }
-    }
+        for (int j = 0; j < PER; ++j) sum1 += expf(-below(top, x[j]));   // nothing for those behind the end
+      }
+      if (k_on || p_on) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (base + j < V) atomicAdd(&s.bins[bin_of(below(top, x[j]), per_bin)], 1u);
+      }
+    });
   float log_sum = 0.f;
   if (out_logprob) {
     double v = (double)sum1;
@@ -346,116 +593,157 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
   }
   __syncthreads();
 
-  u64 floor = 0;
-  if (k_on) {
-    const uint32_t c0 = s.cnt[2 * tid], c1 = s.cnt[2 * tid + 1];
-    u64 all;
-    const u64 after = cta_scan<u64>((u64)c0 + c1, s.red, all);
-    const u64 b0 = after - c0 - c1, b1 = after - c1;
-    if (b0 < (u64)k && (u64)k <= b1) { s.i0 = 2 * tid; s.u0 = b0; }
-    if (b1 < (u64)k && (u64)k <= after) { s.i0 = 2 * tid + 1; s.u0 = b1; }
-    __syncthreads();
-    const int bin = s.i0;
-    const uint32_t before = (uint32_t)s.u0, n = s.cnt[bin];
-    __syncthreads();
-    floor = last_kept<false>(row, s, top, per_bin, inv_t, bin, 0ull, n, (uint32_t)k - before, 0.0);
-    if (p_on) {
-      // the counts of what is left for top-p (dividing a bin may have used the bins)
-      for (int i = tid; i < NB; i += TH) {
-        s.cnt[i] = 0;
-        s.mass[i] = 0;
-      }
-      __syncthreads();
-      for (int c = 0; c < chunks; ++c) {
-        const int base = c * CHUNK + tid * PER;
-        float x[PER];
-        row.get(base, x);
+  // a kept token weighs at least `least`
+  const double least_w = min_p ? ceil(fmax(fmin((double)min_p[b], 1.0), 0.0) * UNIT) : 0.0;
+  const u64 least = (u64)least_w;
+  constexpr int MINE = NB / TH;                                        // bins of a thread
+  uint32_t cnt[MINE];
+  if (k_on || p_on) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-          if (base + j < V && place(x[j], base + j) >= floor) atomicAdd(&s.cnt[bin_of(below(top, x[j]), per_bin)], 1u);
-      }
-      __syncthreads();
-    }
+    for (int i = 0; i < MINE; ++i) cnt[i] = s.bins[MINE * tid + i];
   }
+  int k_bin = NB - 1;
+  uint32_t k_left = 0;                                                 // tokens of k_bin that top-k keeps
+  if (k_on) {
+    u64 sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) sum += cnt[i];
+    u64 before = cta_scan<u64>(sum, s.red, all) - sum;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      if (before < (u64)k && (u64)k <= before + cnt[i]) {
+        s.i0 = MINE * tid + i;
+        s.u0 = before;
+      }
+      before += cnt[i];
+    }
+    __syncthreads();
+    k_bin = s.i0;
+    k_left = (uint32_t)k - (uint32_t)s.u0;
+    __syncthreads();
+  }
+  int from = NB, to = -1;                                              // bins in which top-p can end
   if (p_on) {
     // a bin's weight lies between its count times its least and its largest weight; so do the running sums, and with them the bins in which the
     // sum can reach top_p of the whole
-    const uint32_t c0 = s.cnt[2 * tid], c1 = s.cnt[2 * tid + 1];
-    const float step = RANGE / NB, w0 = __expf(-step * (2 * tid)), fall = __expf(-step);
-    const float h0 = (float)c0 * w0 * 1.0001f, h1 = (float)c1 * w0 * fall * 1.0001f;
-    // the last bin has no least weight
-    const float l0 = (float)c0 * w0 * fall * 0.9999f, l1 = tid == TH - 1 ? 0.f : (float)c1 * w0 * fall * fall * 0.9999f;
-    float most, least;
-    const float ah = cta_scan<float>(h0 + h1, s.fred, most);
-    const float al = cta_scan<float>(l0 + l1, s.fred, least);
+    const float step = RANGE / NB, fall = __expf(-step);
+    float hi[MINE], lo[MINE], hs = 0.f, ls = 0.f, w = __expf(-step * (MINE * tid));
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const int at = MINE * tid + i;
+      const float c = (float)(k_on && at >= k_bin ? at == k_bin ? k_left : 0u : cnt[i]);
+      hi[i] = c * w * 1.0001f;
+      w *= fall;
+      lo[i] = at == NB - 1 ? 0.f : c * w * 0.9999f;                    // the last bin has no least weight
+      hs += hi[i];
+      ls += lo[i];
+    }
+    float most, lowest;
+    float ah = cta_scan<float>(hs, s.fred, most) - hs;
+    float al = cta_scan<float>(ls, s.fred, lowest) - ls;
     const float pp = fmaxf(tp, 0.f);
-    const float lo_goal = pp * least * 0.9999f, hi_goal = pp * most * 1.0001f;
-    if (tid == 0) {
-      s.i0 = NB - 1;
-      s.i1 = NB - 1;
+    const float lo_goal = pp * lowest * 0.9999f, hi_goal = pp * most * 1.0001f;
+    if (tid == 0) s.i0 = s.i1 = k_bin;
+    __syncthreads();
+    bool h_done = false, l_done = false;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      ah += hi[i];
+      al += lo[i];
+      if (!h_done && ah >= lo_goal) { atomicMin(&s.i0, MINE * tid + i); h_done = true; }
+      if (!l_done && al >= hi_goal) { atomicMin(&s.i1, MINE * tid + i); l_done = true; }
     }
     __syncthreads();
-    if (ah - h1 >= lo_goal) atomicMin(&s.i0, 2 * tid);
-    else if (ah >= lo_goal) atomicMin(&s.i0, 2 * tid + 1);
-    if (al - l1 >= hi_goal) atomicMin(&s.i1, 2 * tid);
-    else if (al >= hi_goal) atomicMin(&s.i1, 2 * tid + 1);
+    from = s.i0;
+    to = max(s.i1, from);
     __syncthreads();
-    const int from = s.i0, to = max(s.i1, from);
-    u64 whole = 0, above = 0;
+  }
+  // bins first .. last are looked at token by token; those before are kept, those behind are not (but count for top-p's sum, without top-k)
+  const int first = p_on ? from : k_on ? k_bin : NB, last = k_on ? k_bin : to;
+  const Group by_k{top, per_bin, 0, 0, k_bin};
+  Group by_p{top, per_bin, from, 0, 0};
+  while (((to - from) >> by_p.shift) >= ND) ++by_p.shift;
+  uint32_t n_list = 0;
+  if (first <= last) {
+    u64 c = 0;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i)
+      if (MINE * tid + i >= first && MINE * tid + i <= last) c += cnt[i];
+    n_list = (uint32_t)cta_sum(c, s.red);
+  }
+  if (n_list <= WINDOW) {
+    if (tid == 0) {
+      s.n = 0;
+      s.u0 = 0;
+    }
+    __syncthreads();
+    u64 whole = 0, sure = 0;                                           // weight of everything that top-p's sum counts; of the tokens before `first`
+    const float f_first = (float)first, f_last = last == NB - 1 ? INFINITY : (float)(last + 1);
+    if (k_on) {
+      if (least) weights<false, false, true>(row, s, weigh, f_first, f_last, least, whole, sure);
+      else weights<false, false, false>(row, s, weigh, f_first, f_last, least, whole, sure);
+    } else if (p_on) {
+      if (least) weights<true, true, true>(row, s, weigh, f_first, f_last, least, whole, sure);
+      else weights<true, true, false>(row, s, weigh, f_first, f_last, least, whole, sure);
+    } else {
+      if (least) weights<true, false, true>(row, s, weigh, f_first, f_last, least, whole, sure);
+      else weights<true, false, false>(row, s, weigh, f_first, f_last, least, whole, sure);
+    }
+    __syncthreads();
+    if (first <= last) {
+      const uint32_t n = s.n;
+      u64 floor = 0;
+      if (k_on) {
+        floor = ranked<false>(s, n, by_k, 0ull, k_left, 0.0);
+        if (p_on) {                                                    // of the list, top-p's sum counts what top-k keeps
+          u64 w = 0;
+          for (uint32_t i = tid; i < n; i += TH)
+            if (s.wc[i] >= floor) w += s.ww[i];
+          whole = sure + w;
+        }
+      }
+      if (p_on) {
+        whole = cta_sum(whole, s.red);
+        sure = cta_sum(sure, s.red);
+        for (int i = tid; i < ND; i += TH) s.mass[i] = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += TH)
+          if (s.wc[i] >= floor) {
+            const int g = by_p.of(logit_of(s.wc[i]));
+            if (g < ND) atomicAdd(&s.mass[g], s.ww[i]);
+          }
+        __syncthreads();
+        double want = fmax((double)tp * (double)whole, 0.5) - (double)sure;
+        by_p.g = reached(s, want);
+        if (by_p.g >= 0) floor = ranked<true>(s, n, by_p, floor, 0u, want);      // else nothing is cut
+      }
+      for (uint32_t i = tid; i < n; i += TH)
+        if (s.wc[i] >= floor && s.ww[i] >= least) atomicAdd(&s.cw[(0xffffffffu - (uint32_t)s.wc[i]) / (32 * PER)], s.ww[i]);
+      if (tid == 0) s.u1 = floor;
+    } else if (tid == 0) {
+      s.u1 = 0;
+    }
+  } else {
+    const u64 floor = cut_by_division(row, s, weigh, k_on, by_k, k_left, p_on, by_p, to, tp);
     for (int c = 0; c < chunks; ++c) {
       const int base = c * CHUNK + tid * PER;
       float x[PER];
       row.get(base, x);
+      u64 kept = 0;
 #pragma unroll
       for (int j = 0; j < PER; ++j)
         if (base + j < V && place(x[j], base + j) >= floor) {
-          const u64 w = weight(top, x[j], inv_t);
-          const int bin = bin_of(below(top, x[j]), per_bin);
-          whole += w;
-          if (bin < from) above += w;
-          else if (bin <= to) atomicAdd(&s.mass[bin], w);
+          const u64 w = weigh(x[j]);
+          kept += w >= least ? w : 0;
         }
-    }
-    whole = cta_sum(whole, s.red);
-    above = cta_sum(above, s.red);
-    const double goal = fmax((double)tp * (double)whole, 0.5) - (double)above;
-    const u64 m0 = s.mass[2 * tid], m1 = s.mass[2 * tid + 1];
-    u64 all;
-    const u64 after = cta_scan<u64>(m0 + m1, s.red, all);
-    const u64 b0 = after - m0 - m1, b1 = after - m1;
-    if (tid == 0) s.i0 = -1;
-    __syncthreads();
-    if (m0 && (double)b0 < goal && goal <= (double)b1) { s.i0 = 2 * tid; s.u0 = b0; }
-    if (m1 && (double)b1 < goal && goal <= (double)after) { s.i0 = 2 * tid + 1; s.u0 = b1; }
-    __syncthreads();
-    const int bin = s.i0;
-    if (bin >= 0) {                                                    // else nothing is cut
-      const double want = goal - (double)s.u0;
-      const uint32_t n = s.cnt[bin];
-      __syncthreads();
-      floor = last_kept<true>(row, s, top, per_bin, inv_t, bin, floor, n, 0u, want);
-    }
-  }
-
-  // the draw
-  const double least_w = min_p ? fmin((double)min_p[b], 1.0) * UNIT : 0.0;
-  auto kept = [&](float x, int i) -> u64 {
-    if (i >= V || place(x, i) < floor) return 0;
-    const u64 w = weight(top, x, inv_t);
-    return (double)w >= least_w ? w : 0;
-  };
-  for (int c = 0; c < chunks; ++c) {
-    const int base = c * CHUNK + tid * PER;
-    float x[PER];
-    row.get(base, x);
-    u64 w = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) w += kept(x[j], base + j);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    if (lane == 0) s.cw[c * 32 + warp] = w;
+      for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
+      if (lane == 0) s.cw[c * 32 + warp] = kept;
+    }
+    if (tid == 0) s.u1 = floor;
   }
   __syncthreads();
+  const u64 floor = s.u1;
   const u64 mine = tid < chunks * 32 ? s.cw[tid] : 0;
   u64 all;
   const u64 upto = cta_scan<u64>(mine, s.red, all);
@@ -476,7 +764,8 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
     u64 w[PER], sum = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      w[j] = kept(x[j], base + j);
+      w[j] = base + j < V && place(x[j], base + j) >= floor ? weigh(x[j]) : 0;
+      if (w[j] < least) w[j] = 0;
       sum += w[j];
     }
     u64 at = s.u0 + warp_scan(sum) - sum;

@@ -213,6 +213,10 @@ def splits8(ctas: int, reach: int) -> int:
     should save), 64 tokens at least. Up to 8 are one cluster, more are clusters of one size. us, 4 rows of 30011 tokens with 8 key heads: 6 splits
     72, 8 59, 12 57, 16 (two waves) 70; 32 rows of 4000 tokens with 4 key heads: 1 split 49, 2 41, 3 37, 4 (two waves) 49."""
     n = max(1, min(128, 3 * 148 // max(1, ctas), -(-reach // 64)))
+    # 9 .. 15 of short contexts: one cluster and no kernel to join two (700 tokens with 32 key heads: 19 us in 10 splits, 15 in 8; but 4 rows of
+    # 30011 tokens with 8 key heads: 47 us in 12, 61 in 8)
+    if n < 16 and reach <= 4096:
+        return min(n, 8)
     while n % -(-n // 8):
         n -= 1
     return n
