@@ -21,11 +21,11 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int TH = 1024, PER = 8;                 // threads, and consecutive tokens of a thread in a chunk
+constexpr int TH = 512, WARPS = TH / 32, PER = 8; // threads, and consecutive tokens of a thread in a chunk
 constexpr int CHUNK = TH * PER;
-constexpr int NB = 8 * TH, ND = 2 * TH;            // bins of the distance from the largest; digits of 11 bits
+constexpr int NB = 8192, ND = 2048;               // bins of the distance from the largest; digits of 11 bits
 constexpr int LIST = 512, WINDOW = 7168;
-constexpr int V_MAX = 1 << 18;
+constexpr int V_MAX = 1 << 18, GROUPS = V_MAX / (32 * PER);
 constexpr double UNIT = 35184372088832.0;         // 2^45
 constexpr float RANGE = 32.f;                     // bins reach this far below the largest logit, in units of T: e^-32 < 2^-46
 
@@ -41,7 +41,7 @@ struct Work {
       u64 wc[WINDOW], ww[WINDOW];                 // tokens of all bins in which a cut may lie
     };
   };
-  u64 cw[V_MAX / (32 * PER)];
+  u64 cw[GROUPS];                                 // kept weight of 256 tokens each
   u64 red[32];
   float fred[32];
   u64 u0, u1;
@@ -178,7 +178,7 @@ __device__ __forceinline__ S cta_scan(S v, S* red, S& total) {
   __syncthreads();
   if ((threadIdx.x & 31) == 31) red[w] = v;
   __syncthreads();
-  const S mine = warp_scan(red[threadIdx.x & 31]);
+  const S mine = warp_scan((threadIdx.x & 31) < WARPS ? red[threadIdx.x & 31] : S(0));
   const S before = __shfl_sync(0xffffffffu, mine, w ? w - 1 : 0);
   total = __shfl_sync(0xffffffffu, mine, 31);
   return v + (w ? before : S(0));
@@ -189,26 +189,39 @@ __device__ __forceinline__ u64 cta_sum(u64 v, u64* red) {
   return total;
 }
 
-// Which of the counted digits (s.cnt, s.mass; s.i0 = -1) the cut lies in: the last one that is there, if sums fall short of it. What lies before it is
-// taken from r or `want`.
+// The i-th of n running sums in which `goal` lies (before < goal <= after, of values that are there) to s.i0, what comes before it to s.u0; s.i0 stays
+// as it is if there is none. A thread looks at n / TH neighbours. Returns the whole sum.
+template <int N, typename V>
+__device__ __forceinline__ u64 find(Work& s, V&& value, double goal) {
+  constexpr int E = N / TH;
+  u64 v[E], sum = 0, all;
+#pragma unroll
+  for (int i = 0; i < E; ++i) sum += v[i] = value(E * threadIdx.x + i);
+  u64 before = cta_scan<u64>(sum, s.red, all) - sum;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (v[i] && (double)before < goal && goal <= (double)(before + v[i])) {
+      s.i0 = E * threadIdx.x + i;
+      s.u0 = before;
+    }
+    before += v[i];
+  }
+  __syncthreads();
+  return all;
+}
+// Which of the counted digits (s.cnt, s.mass) the cut lies in: the last one that is there, if sums fall short of it. What lies before it is taken from r
+// or `want`.
 template <bool MASS>
 __device__ __forceinline__ int digit(Work& s, uint32_t& r, double& want) {
-  const int tid = threadIdx.x;
-  const uint32_t c0 = s.cnt[2 * tid], c1 = s.cnt[2 * tid + 1];
-  const u64 v0 = MASS ? s.mass[2 * tid] : c0, v1 = MASS ? s.mass[2 * tid + 1] : c1;
-  u64 all;
-  const u64 after = cta_scan<u64>(v0 + v1, s.red, all);
-  const u64 b0 = after - v0 - v1, b1 = after - v1;
-  const double capped = fmin(MASS ? want : (double)r, (double)all);
-  if (c0 && (double)b0 < capped && capped <= (double)b1) { s.i0 = 2 * tid; s.u0 = b0; }
-  if (c1 && (double)b1 < capped && capped <= (double)after) { s.i0 = 2 * tid + 1; s.u0 = b1; }
+  if (threadIdx.x == 0) s.i0 = -1;
   __syncthreads();
+  const u64 all = find<ND>(s, [&](int i) { return MASS ? s.mass[i] : (u64)s.cnt[i]; }, MASS ? want : (double)r);
   const bool none = s.i0 < 0;
   __syncthreads();
-  if (none) {                                                          // no weight at all: everything is kept up to the last token there is
-    if (c0) atomicMax(&s.i0, 2 * tid);
-    if (c1) atomicMax(&s.i0, 2 * tid + 1);
-    if (tid == 0) s.u0 = all;
+  if (none) {                                                          // everything is kept, up to the last token there is
+    for (int i = threadIdx.x; i < ND; i += TH)
+      if (s.cnt[i]) atomicMax(&s.i0, i);
+    if (threadIdx.x == 0) s.u0 = MASS ? all : all - 1;
     __syncthreads();
   }
   if (MASS) want -= (double)s.u0;
@@ -251,7 +264,6 @@ __device__ __noinline__ u64 last_kept(const Row<T> row, Work& s, const Weigh wei
         if (MASS) atomicAdd(&s.mass[d], weigh(x));
       }
     });
-    if (tid == 0) s.i0 = -1;
     __syncthreads();
     const int at = digit<MASS>(s, r, want);
     n = s.cnt[at];
@@ -299,7 +311,6 @@ __device__ __noinline__ u64 last_kept(const Row<T> row, Work& s, const Weigh wei
     r = w > 0 ? (uint32_t)fmin(fmax(ceil(want / w), 1.0), (double)n) : n;
   }
   r = min(max(r, 1u), n);
-  const int groups = chunks * 32;
   for (int c = 0; c < chunks; ++c) {
     const int base = c * CHUNK + tid * PER;
     float x[PER];
@@ -309,20 +320,13 @@ __device__ __noinline__ u64 last_kept(const Row<T> row, Work& s, const Weigh wei
     for (int j = 0; j < PER; ++j)
       k += base + j < row.V && key_of(x[j]) == prefix && place(x[j], base + j) >= floor;
     k = __reduce_add_sync(0xffffffffu, k);
-    if ((tid & 31) == 0) s.cw[c * 32 + (tid >> 5)] = k;
+    if ((tid & 31) == 0) s.cw[c * WARPS + (tid >> 5)] = k;
   }
   __syncthreads();
-  const u64 mine = tid < groups ? s.cw[tid] : 0;
-  u64 all;
-  const u64 upto = cta_scan<u64>(mine, s.red, all);
-  if (upto - mine < r && r <= upto) {
-    s.i0 = tid;
-    s.u0 = upto - mine;
-  }
-  __syncthreads();
+  find<GROUPS>(s, [&](int i) { return i < chunks * WARPS ? s.cw[i] : 0; }, (double)r);
   const int g = s.i0;
-  if ((tid >> 5) == (g & 31)) {
-    const int base = (g >> 5) * CHUNK + tid * PER;
+  if ((tid >> 5) == g % WARPS) {
+    const int base = g / WARPS * CHUNK + tid * PER;
     float x[PER];
     row.get(base, x);
     uint32_t k = 0;
@@ -369,7 +373,6 @@ __device__ __noinline__ u64 ranked(Work& s, uint32_t n, const Group group, u64 f
       s.cnt[i] = 0;
       s.mass[i] = 0;
     }
-    if (tid == 0) s.i0 = -1;
     __syncthreads();
     for (uint32_t i = tid; i < n; i += TH) {
       const u64 c = s.wc[i];
@@ -409,16 +412,9 @@ __device__ __noinline__ u64 ranked(Work& s, uint32_t n, const Group group, u64 f
 
 // Where top-p ends: the group in which the weights (s.mass, by group) reach `goal`, -1 if they do not; what is left of goal there.
 __device__ __forceinline__ int reached(Work& s, double& goal) {
-  const int tid = threadIdx.x;
-  const u64 m0 = s.mass[2 * tid], m1 = s.mass[2 * tid + 1];
-  u64 all;
-  const u64 after = cta_scan<u64>(m0 + m1, s.red, all);
-  const u64 b0 = after - m0 - m1, b1 = after - m1;
-  if (tid == 0) s.i0 = -1;
+  if (threadIdx.x == 0) s.i0 = -1;
   __syncthreads();
-  if (m0 && (double)b0 < goal && goal <= (double)b1) { s.i0 = 2 * tid; s.u0 = b0; }
-  if (m1 && (double)b1 < goal && goal <= (double)after) { s.i0 = 2 * tid + 1; s.u0 = b1; }
-  __syncthreads();
+  find<ND>(s, [&](int i) { return s.mass[i]; }, goal);
   const int g = s.i0;
   if (g >= 0) goal -= (double)s.u0;
   __syncthreads();
@@ -498,7 +494,7 @@ __device__ __noinline__ void weights(const Row<T> row, Work& s, const Weigh weig
     if (!CUT) sure += kept;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
-    if ((threadIdx.x & 31) == 0) s.cw[c * 32 + (threadIdx.x >> 5)] = kept;
+    if ((threadIdx.x & 31) == 0) s.cw[c * WARPS + (threadIdx.x >> 5)] = kept;
   });
   whole_ = whole;
   sure_ = sure;
@@ -532,7 +528,7 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (lane == 0) s.red[warp] = best;
   __syncthreads();
-  best = s.red[lane];
+  best = lane < WARPS ? s.red[lane] : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   const int arg = (int)(0xffffffffu - (uint32_t)best);
@@ -579,7 +575,7 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lane == 0) s.red[warp] = __double_as_longlong(v);
     __syncthreads();
-    v = __longlong_as_double(s.red[lane]);
+    v = lane < WARPS ? __longlong_as_double(s.red[lane]) : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     log_sum = (float)log(v);
@@ -738,27 +734,33 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
         }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
-      if (lane == 0) s.cw[c * 32 + warp] = kept;
+      if (lane == 0) s.cw[c * WARPS + warp] = kept;
     }
     if (tid == 0) s.u1 = floor;
   }
   __syncthreads();
   const u64 floor = s.u1;
-  const u64 mine = tid < chunks * 32 ? s.cw[tid] : 0;
-  u64 all;
-  const u64 upto = cta_scan<u64>(mine, s.red, all);
+  constexpr int E = GROUPS / TH;
+  u64 group[E], sum = 0, all;
+#pragma unroll
+  for (int i = 0; i < E; ++i) sum += group[i] = E * tid + i < chunks * WARPS ? s.cw[E * tid + i] : 0;
+  u64 before = cta_scan<u64>(sum, s.red, all) - sum;
   // a number that rounding takes to the whole sum falls on the last token
   const double goal = fmin(fmax(u[b], 0.0) * (double)all, (double)all * (1.0 - 2.3e-16));
   if (tid == 0) s.i0 = 0;
   __syncthreads();
-  if (mine && (double)(upto - mine) <= goal && goal < (double)upto) {
-    s.i0 = tid;
-    s.u0 = upto - mine;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (group[i] && (double)before <= goal && goal < (double)(before + group[i])) {
+      s.i0 = E * tid + i;
+      s.u0 = before;
+    }
+    before += group[i];
   }
   __syncthreads();
   const int g = s.i0;
-  if (warp == (g & 31)) {
-    const int base = (g >> 5) * CHUNK + tid * PER;
+  if (warp == g % WARPS) {
+    const int base = g / WARPS * CHUNK + tid * PER;
     float x[PER];
     row.get(base, x);
     u64 w[PER], sum = 0;
