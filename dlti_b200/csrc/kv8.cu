@@ -57,9 +57,11 @@ __device__ __forceinline__ int4 pack8(const float (&f)[8]) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Rows of a step. Sixteen lanes hold one head of one row, 8 elements each; the element that a rotation pairs with is 8 lanes away.
-// A warp takes the rows of one page (consecutive rows with slots in it) for one key or value head, so nobody else touches that head's piece
-// of the page or its scale. Query heads are only rotated: a warp takes up to 8 of a row.
+// Rows of a step. Sixteen lanes hold one head of one row, 8 elements each; the element that a rotation pairs with is 8 lanes away, and a warp
+// has two rows at a time. A CTA takes a block of rows, whose angles it keeps in shared memory in the rows' type, and a share of the heads. Of
+// keys and values a warp takes all rows of one page (consecutive rows with slots in it) for one head, so nobody else touches that head's piece of
+// the page or its scale; a page that goes on behind the block is done by the CTA in whose block it begins. Up to 16 rows are in flight and stay in
+// registers between finding the scale and rounding to it.
 // ---------------------------------------------------------------------------------------------
 struct Rows8 {
   const void* x;                 // [tokens, x_ld] in the rows' type, or the fp32 accumulator [tokens, (H + 2 KV) * 128], left zero
@@ -86,172 +88,205 @@ __device__ __forceinline__ int4 take(const Rows8& p, long long t, int h, int l16
     return *reinterpret_cast<const int4*>(reinterpret_cast<const T*>(p.x) + t * p.x_ld + h * HD + l16 * 8);
   }
 }
+// ROWS of a block, KEEP pairs of rows that a warp has in flight and keeps in registers. Decode steps: 1 and 1, a row is a page of its own.
+template <int ROWS_, int KEEP_, int CTAS_>
+struct RowsCfg {
+  static constexpr int ROWS = ROWS_, KEEP = KEEP_, CTAS = CTAS_;
+};
+using DecodeRows = RowsCfg<1, 1, 4>;
+using PromptRows = RowsCfg<16, 8, 3>;
+
+// cosines and sines of row t in the rows' type, rounded as the 16-bit cache's ops round them
 template <typename T>
-__device__ __forceinline__ void angles(const Rows8& p, long long t, int l16, float (&c)[8], float (&s)[8]) {
-  const long long at = (long long)p.pos[t] * (HD / 2) + (l16 & 7) * 8;
-  const float4 c0 = *reinterpret_cast<const float4*>(p.cos_t + at), c1 = *reinterpret_cast<const float4*>(p.cos_t + at + 4);
-  const float4 s0 = *reinterpret_cast<const float4*>(p.sin_t + at), s1 = *reinterpret_cast<const float4*>(p.sin_t + at + 4);
-  const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    c[j] = Cvt<T>::to_f(Cvt<T>::from_f(cc[j]));
-    const float v = Cvt<T>::to_f(Cvt<T>::from_f(ss[j]));
-    s[j] = l16 < 8 ? -v : v;
-  }
+struct Angles {
+  int4 c, s;
+};
+template <typename T>
+__device__ __forceinline__ int4 rounded8(const float* f) {
+  const float4 a = *reinterpret_cast<const float4*>(f), b = *reinterpret_cast<const float4*>(f + 4);
+  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  return pack8<T>(v);
 }
 // The lane's 8 elements rotated (all lanes of the warp call). Products of two 16-bit numbers are exact in fp32, so one rounding is left.
 template <typename T>
-__device__ __forceinline__ int4 turn(const int4& v, const float (&c)[8], const float (&s)[8]) {
+__device__ __forceinline__ int4 turn(const int4& v, const Angles<T>& an, bool low) {
   int4 w;
   w.x = __shfl_xor_sync(0xffffffffu, v.x, 8);
   w.y = __shfl_xor_sync(0xffffffffu, v.y, 8);
   w.z = __shfl_xor_sync(0xffffffffu, v.z, 8);
   w.w = __shfl_xor_sync(0xffffffffu, v.w, 8);
-  float a[8], b[8];
+  if (low) w = make_int4(w.x ^ 0x80008000, w.y ^ 0x80008000, w.z ^ 0x80008000, w.w ^ 0x80008000);
+  float a[8], b[8], c[8], s[8];
   unpack8<T>(v, a);
   unpack8<T>(w, b);
+  unpack8<T>(an.c, c);
+  unpack8<T>(an.s, s);
 #pragma unroll
   for (int j = 0; j < 8; ++j) a[j] = a[j] * c[j] + b[j] * s[j];
   return pack8<T>(a);
 }
 
-constexpr int KEEP = 8;          // pairs of rows that a warp keeps in registers between finding the scale and rounding to it
-
-template <typename T, bool ACC>
-__global__ void __launch_bounds__(256) rows8_kernel(const Rows8 p, int block, int q_units) {
+template <typename T, bool ACC, typename C>
+__global__ void __launch_bounds__(256, C::CTAS) rows8_kernel(const Rows8 p) {
+  constexpr int block = C::ROWS, KEEP = C::KEEP, STAGED = block == 1 ? 1 : 2 * block;
   griddep_pass(p.tokens);
-  const int lane = threadIdx.x & 31, l16 = lane & 15, half = lane >> 4;
-  const int blocks = (p.tokens + block - 1) / block;
-  const long long kv_units = (long long)blocks * 2 * p.KV;
-  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const bool copy = ACC || p.out != p.x;
+  __shared__ int4 s_angle[STAGED][16];                    // of a row: 8 pieces of cosines, 8 of sines
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l16 = lane & 15, half = lane >> 4;
+  const int first = blockIdx.x * block, last = min(p.tokens, first + block);
+  const int staged = min(p.tokens - first, STAGED);
+  const bool copy = ACC || p.out != p.x, low = l16 < 8;
   T* out = reinterpret_cast<T*>(p.out);
-  if (unit >= kv_units) {                                   // rotate up to 8 query heads of a row
-    const long long u = unit - kv_units;
-    const long long t = u / q_units;
-    if (t >= p.tokens) return;
-    const int h0 = (int)(u - t * q_units) * 8 + half;
-    int4 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (h0 + 2 * i < p.H) v[i] = take<T, ACC>(p, t, h0 + 2 * i, l16);
-      else v[i] = make_int4(0, 0, 0, 0);
-    float c[8], s[8];
-    angles<T>(p, t, l16, c, s);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int4 r = turn<T>(v[i], c, s);
-      if (h0 + 2 * i < p.H) *reinterpret_cast<int4*>(out + t * p.out_ld + (h0 + 2 * i) * HD + l16 * 8) = r;
-    }
-    return;
+  for (int i = threadIdx.x; i < staged * 16; i += 256) {
+    const long long at = (long long)p.pos[first + (i >> 4)] * (HD / 2) + (i & 7) * 8;
+    s_angle[i >> 4][i & 15] = rounded8<T>((i & 8 ? p.sin_t : p.cos_t) + at);
   }
-  const int hh = (int)(unit % (2 * p.KV));                  // key heads, then value heads
-  const bool key = hh < p.KV;
-  const int head = key ? hh : hh - p.KV;
-  const int col = p.H + hh;
-  uint8_t* cache = key ? p.k8 : p.v8;
-  float* scales = key ? p.ks : p.vs;
-  const int first = (int)(unit / (2 * p.KV)) * block, last = min(p.tokens, first + block);
-  auto page_of = [&](int t) { const long long s = p.slots[t]; return s < 0 ? -1 : (int)((uint32_t)s / (uint32_t)p.bs); };
-  for (int t = first; t < last;) {
-    const int page = page_of(t);
-    if (page >= 0 && t == first && t > 0 && page_of(t - 1) == page) {   // these rows belong to the warp of the rows before
-      while (t < last && page_of(t) == page) ++t;
-      continue;
+  __syncthreads();
+  auto angles = [&](int t) {
+    Angles<T> a;
+    if (t - first < staged) {
+      a.c = s_angle[t - first][l16 & 7];
+      a.s = s_angle[t - first][8 + (l16 & 7)];
+    } else {
+      const long long at = (long long)p.pos[t] * (HD / 2) + (l16 & 7) * 8;
+      a.c = rounded8<T>(p.cos_t + at);
+      a.s = rounded8<T>(p.sin_t + at);
     }
-    // the run [t, t + n) of rows of this page; a row without a slot is by itself
-    int n = 1;
-    bool fresh = false;
-    if (page >= 0) {
-      fresh = (uint32_t)p.slots[t] % (uint32_t)p.bs == 0;
-      for (;;) {
-        const int r = t + n + lane;
-        const long long s = r < p.tokens ? p.slots[r] : -1;
-        const bool in = s >= 0 && (int)((uint32_t)s / (uint32_t)p.bs) == page;
-        const uint32_t out_of = ~__ballot_sync(0xffffffffu, in);
-        const int more = out_of ? __ffs(out_of) - 1 : 32;
-        fresh |= __any_sync(0xffffffffu, in && lane < more && (uint32_t)s % (uint32_t)p.bs == 0);
-        n += more;
-        if (more < 32) break;
-      }
-    }
+    return a;
+  };
+  auto put_out = [&](int t, int col, const int4& v) { *reinterpret_cast<int4*>(out + t * p.out_ld + col * HD + l16 * 8) = v; };
+  const int heads = p.H + 2 * p.KV;
+  for (int col = blockIdx.y * 8 + warp; col < heads; col += gridDim.y * 8) {
     int4 held[KEEP];
-    float largest = 0.f;
-    auto see = [&](int r, bool keep, int i) {
-      const bool ok = r < n;
-      const long long row = t + (ok ? r : 0);
-      int4 v = make_int4(0, 0, 0, 0);
-      if (ok) v = take<T, ACC>(p, row, col, l16);
-      if (key) {
-        float c[8], s[8];
-        angles<T>(p, row, l16, c, s);
-        v = turn<T>(v, c, s);
-      }
-      if (ok && (key || copy)) *reinterpret_cast<int4*>(out + row * p.out_ld + col * HD + l16 * 8) = v;
-      float f[8];
-      unpack8<T>(v, f);
+    // rows t + 16 k ... of a run of n
+    auto request = [&](int t, int n) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = fabsf(f[j]);
-        if (ok && a < INFINITY) largest = fmaxf(largest, a);          // neither infinities nor NaN set the scale
+      for (int i = 0; i < KEEP; ++i) {
+        held[i] = make_int4(0, 0, 0, 0);
+        if (2 * i + half < n) held[i] = take<T, ACC>(p, t + 2 * i + half, col, l16);
       }
-      return v;
     };
+    if (col < p.H) {                                        // a query head
+      for (int at = first; at < last; at += 2 * KEEP) {
+        request(at, last - at);
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i)
-      if (2 * i < n) held[i] = see(2 * i + half, true, i);
-    for (int r = 2 * KEEP; r < n; r += 2) see(r + half, false, 0);
-    if (page >= 0) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-      const long long sc = (long long)page * p.KV + head;
-      uint8_t* piece = cache + sc * p.bs * HD;
-      const float old = fresh ? pow2i(E_LOW) : scales[sc];
-      const float now = fmaxf(old, scale_for(largest));
-      if (!fresh && now > old) {                            // what the page holds is rounded to the new scale
-        const float ratio = old / now;
-        for (int i = lane; i < p.bs * (HD / 16); i += 32) {
-          int4 v = reinterpret_cast<const int4*>(piece)[i];
-          uint32_t* u = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 a = float2_of_e4m3x2(u[j] & 0xffffu), b = float2_of_e4m3x2(u[j] >> 16);
-            u[j] = e4m3x2(a.x * ratio, a.y * ratio) | e4m3x2(b.x * ratio, b.y * ratio) << 16;
-          }
-          reinterpret_cast<int4*>(piece)[i] = v;
+        for (int i = 0; i < KEEP; ++i) {
+          const int t = at + 2 * i + half;
+          if (at + 2 * i >= last) break;
+          const int4 v = turn<T>(held[i], angles(min(t, last - 1)), low);
+          if (t < last) put_out(t, col, v);
         }
       }
-      __syncwarp();
-      if (lane == 0) scales[sc] = now;
-      const float inv = 1.f / now;
-      auto put = [&](int r, const int4& v) {
-        if (r >= n) return;
-        float f[8];
-        unpack8<T>(v, f);
-        uint2 o;
-        o.x = e4m3x2(f[0] * inv, f[1] * inv) | e4m3x2(f[2] * inv, f[3] * inv) << 16;
-        o.y = e4m3x2(f[4] * inv, f[5] * inv) | e4m3x2(f[6] * inv, f[7] * inv) << 16;
-        const uint32_t off = (uint32_t)p.slots[t + r] % (uint32_t)p.bs;
-        *reinterpret_cast<uint2*>(piece + off * HD + l16 * 8) = o;
-      };
-#pragma unroll
-      for (int i = 0; i < KEEP; ++i)
-        if (2 * i < n) put(2 * i + half, held[i]);
-      for (int r = 2 * KEEP + half; r < n; r += 2)          // longer pages: this lane wrote (or, without a copy, read) these pieces itself
-        put(r, *reinterpret_cast<const int4*>(out + (long long)(t + r) * p.out_ld + col * HD + l16 * 8));
+      continue;
     }
-    t += n;
+    const int hh = col - p.H;                               // key heads, then value heads
+    const bool key = hh < p.KV;
+    const int head = key ? hh : hh - p.KV;
+    uint8_t* cache = key ? p.k8 : p.v8;
+    float* scales = key ? p.ks : p.vs;
+    const uint32_t bs = p.bs;
+    auto page_of = [&](int t) { const long long s = p.slots[t]; return s < 0 ? -1 : (int)((uint32_t)s / bs); };
+    for (int t = first; t < last;) {
+      const int page = page_of(t);
+      if (page >= 0 && t == first && t > 0 && page_of(t - 1) == page) {   // these rows belong to the block before
+        while (t < last && page_of(t) == page) ++t;
+        continue;
+      }
+      // the run [t, t + n) of rows of this page; a row without a slot is by itself. Lane i < 32 looks at row t + i
+      int n = 1;
+      bool fresh = false;
+      uint32_t off = 0;                                     // place of row t + lane
+      if (page >= 0) {
+        for (int k = 0;; k += 32) {
+          const int r = t + k + lane;
+          const long long s = r < p.tokens ? p.slots[r] : -1;
+          const bool in = s >= 0 && (int)((uint32_t)s / bs) == page;
+          const uint32_t place = (uint32_t)s - (uint32_t)page * bs;
+          if (k == 0) off = place;
+          const uint32_t out_of = ~__ballot_sync(0xffffffffu, in);
+          const int more = out_of ? __ffs(out_of) - 1 : 32;
+          fresh |= __any_sync(0xffffffffu, in && lane < more && place == 0);
+          n = k + more;
+          if (more < 32) break;
+        }
+      }
+      const long long sc = (long long)page * p.KV + head;
+      float old = pow2i(E_LOW);
+      if (page >= 0 && !fresh) old = scales[sc];
+      float largest = 0.f;
+      for (int k = 0; k < n; k += 2 * KEEP) {
+        request(t + k, n - k);
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) {
+          if (k + 2 * i >= n) break;
+          const int r = k + 2 * i + half;
+          if (key) held[i] = turn<T>(held[i], angles(t + min(r, n - 1)), low);
+          if (r < n && (key || copy)) put_out(t + r, col, held[i]);
+          float f[8];
+          unpack8<T>(held[i], f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float a = fabsf(f[j]);
+            largest = fmaxf(largest, a < INFINITY ? a : 0.f);             // neither infinities nor NaN set the scale; rows that are not there are 0
+          }
+        }
+      }
+      if (page >= 0) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        uint8_t* piece = cache + sc * bs * HD;
+        const float now = fmaxf(old, scale_for(largest));
+        if (!fresh && now > old) {                          // what the page holds is rounded to the new scale
+          const float ratio = old / now;
+          for (int i = lane; i < (int)bs * (HD / 16); i += 32) {
+            int4 v = reinterpret_cast<const int4*>(piece)[i];
+            uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 a = float2_of_e4m3x2(u[j] & 0xffffu), b = float2_of_e4m3x2(u[j] >> 16);
+              u[j] = e4m3x2(a.x * ratio, a.y * ratio) | e4m3x2(b.x * ratio, b.y * ratio) << 16;
+            }
+            reinterpret_cast<int4*>(piece)[i] = v;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) scales[sc] = now;
+        const float inv = 1.f / now;
+        auto put = [&](uint32_t place, const int4& v) {
+          float f[8];
+          unpack8<T>(v, f);
+          uint2 o;
+          o.x = e4m3x2(f[0] * inv, f[1] * inv) | e4m3x2(f[2] * inv, f[3] * inv) << 16;
+          o.y = e4m3x2(f[4] * inv, f[5] * inv) | e4m3x2(f[6] * inv, f[7] * inv) << 16;
+          *reinterpret_cast<uint2*>(piece + place * HD + l16 * 8) = o;
+        };
+        if (n <= 2 * KEEP) {
+#pragma unroll
+          for (int i = 0; i < KEEP; ++i) {
+            const uint32_t place = __shfl_sync(0xffffffffu, off, 2 * i + half);
+            if (2 * i + half < n) put(place, held[i]);
+          }
+        } else {                                            // longer pages: this lane wrote (or, without a copy, read) these pieces itself
+          for (int r = half; r < n; r += 2)
+            put((uint32_t)p.slots[t + r] - (uint32_t)page * bs, *reinterpret_cast<const int4*>(out + (long long)(t + r) * p.out_ld + col * HD + l16 * 8));
+        }
+      }
+      t += n;
+    }
   }
 }
 
 template <typename T, bool ACC>
 int rows8_t(const Rows8& p, cudaStream_t st) {
-  const int q_units = (p.H + 7) / 8;
-  // one row a warp while all of them fit the GPU at once (the rows of a decode step are pages of their own), else 16: most rows of a prompt
-  // belong to the warp of a row before
-  const int block = (long long)p.tokens * 2 * p.KV <= 148 * 64 ? 1 : 16;
-  const long long units = (long long)((p.tokens + block - 1) / block) * 2 * p.KV + (long long)p.tokens * q_units;
-  DLTI_CUDA_CHECK(dlti_launch_pdl(p.tokens, rows8_kernel<T, ACC>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, st, p, block, q_units));
+  const int heads = p.H + 2 * p.KV, eights = (heads + 7) / 8;
+  if (p.tokens <= DLTI_PDL_MAX_ROWS) {
+    DLTI_CUDA_CHECK(dlti_launch_pdl(p.tokens, rows8_kernel<T, ACC, DecodeRows>, dim3((unsigned)p.tokens, (unsigned)eights), dim3(256), 0, st, p));
+  } else {
+    const int blocks = (p.tokens + PromptRows::ROWS - 1) / PromptRows::ROWS;
+    const long long ctas = (long long)blocks * eights;
+    const int share = ctas <= 3 * 148 ? 1 : ctas <= 10 * 148 ? 2 : 4;      // heads of a warp
+    DLTI_CUDA_CHECK(dlti_launch_pdl(p.tokens, rows8_kernel<T, ACC, PromptRows>, dim3((unsigned)blocks, (unsigned)((eights + share - 1) / share)), dim3(256),
+                                    0, st, p));
+  }
   dlti_count_launch();
   return 0;
 }
@@ -687,27 +722,40 @@ int attend8_t(const Attend8& p, int batch, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Cached rows in 16 bits: row rows[i] of ext gets the keys and values of slot slots[i] at its key and value columns. A thread takes 8 numbers.
+// Cached rows in 16 bits: row rows[i] of ext gets the keys and values of slot slots[i] at its key and value columns. A warp takes 16 heads of one
+// row, 8 numbers a lane and load, all eight loads before the first store.
 // ---------------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) gather8_kernel(T* __restrict__ ext, long long ext_ld, const long long* __restrict__ rows,
                                                       const long long* __restrict__ slots, const uint8_t* __restrict__ k8,
                                                       const uint8_t* __restrict__ v8, const float* __restrict__ ks, const float* __restrict__ vs,
-                                                      long long n, int H, int KV, int bs) {
-  const long long total = n * 2 * KV * 16;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const int c = (int)(i & 15);
-    const long long u = i >> 4;
-    const long long r = u / (2 * KV);
-    const int hh = (int)(u - r * 2 * KV);
-    const bool key = hh < KV;
-    const uint32_t slot = (uint32_t)slots[r], page = slot / (uint32_t)bs, off = slot - page * bs;
-    const long long sc = (long long)page * KV + (key ? hh : hh - KV);
-    const uint2 v = *reinterpret_cast<const uint2*>((key ? k8 : v8) + (sc * bs + off) * HD + c * 8);
-    const float s = (key ? ks : vs)[sc];
-    const float2 a = float2_of_e4m3x2(v.x & 0xffffu), b = float2_of_e4m3x2(v.x >> 16), d = float2_of_e4m3x2(v.y & 0xffffu), e = float2_of_e4m3x2(v.y >> 16);
-    const float f[8] = {a.x * s, a.y * s, b.x * s, b.y * s, d.x * s, d.y * s, e.x * s, e.y * s};
-    *reinterpret_cast<int4*>(ext + rows[r] * ext_ld + (long long)(H + hh) * HD + c * 8) = pack8<T>(f);
+                                                      int n, int H, int KV, int bs) {
+  const int lane = threadIdx.x & 31, c = (lane & 15) * 8;
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), h0 = blockIdx.y * 16 + (lane >> 4);
+  if (r >= n) return;
+  const uint32_t slot = (uint32_t)slots[r], page = slot / (uint32_t)bs, off = slot - page * bs;
+  T* dst = ext + rows[r] * ext_ld + (long long)H * HD + c;
+  uint2 v[8];
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int hh = h0 + 2 * i;
+    if (hh < 2 * KV) {
+      const bool key = hh < KV;
+      const uint32_t sc = page * KV + (key ? hh : hh - KV);
+      v[i] = *reinterpret_cast<const uint2*>((key ? k8 : v8) + ((unsigned long long)sc * bs + off) * HD + c);
+      s[i] = (key ? ks : vs)[sc];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int hh = h0 + 2 * i;
+    if (hh < 2 * KV) {
+      const float2 a = float2_of_e4m3x2(v[i].x & 0xffffu), b = float2_of_e4m3x2(v[i].x >> 16), d = float2_of_e4m3x2(v[i].y & 0xffffu),
+                   e = float2_of_e4m3x2(v[i].y >> 16);
+      const float f[8] = {a.x * s[i], a.y * s[i], b.x * s[i], b.y * s[i], d.x * s[i], d.y * s[i], e.x * s[i], e.y * s[i]};
+      *reinterpret_cast<int4*>(dst + hh * HD) = pack8<T>(f);
+    }
   }
 }
 
@@ -773,12 +821,12 @@ DLTI_API int dlti_gather_rows8(void* ext, long long ext_ld, const long long* row
                                const float* ks, const float* vs, long long n, int H, int KV, int hd, int bs, int dtype, cudaStream_t st) {
   if (!sizes_ok("gather_rows8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
   if (n <= 0) return 0;
-  const long long need = (n * 2 * KV * 16 + 255) / 256, cap = (long long)dlti_num_sms() * 64;
-  const unsigned grid = (unsigned)(need < cap ? need : cap);
+  if (n > 1 << 30) return DLTI_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)((n + 7) / 8), (unsigned)((2 * KV + 15) / 16));
   if (dtype == DLTI_BF16)
-    gather8_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((__nv_bfloat16*)ext, ext_ld, rows, slots, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, n, H, KV, bs);
+    gather8_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((__nv_bfloat16*)ext, ext_ld, rows, slots, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, (int)n, H, KV, bs);
   else if (dtype == DLTI_FP16)
-    gather8_kernel<__half><<<grid, 256, 0, st>>>((__half*)ext, ext_ld, rows, slots, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, n, H, KV, bs);
+    gather8_kernel<__half><<<grid, 256, 0, st>>>((__half*)ext, ext_ld, rows, slots, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, (int)n, H, KV, bs);
   else
     return DLTI_ERR_UNSUPPORTED;
   dlti_count_launch();
