@@ -659,13 +659,15 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
   const Group by_k{top, per_bin, 0, 0, k_bin};
   Group by_p{top, per_bin, from, 0, 0};
   while (((to - from) >> by_p.shift) >= ND) ++by_p.shift;
-  uint32_t n_list = 0;
+  uint32_t n_list = 0, n_before = 0;                                   // their tokens, and those before them
   if (first <= last) {
     u64 c = 0;
 #pragma unroll
     for (int i = 0; i < MINE; ++i)
-      if (MINE * tid + i >= first && MINE * tid + i <= last) c += cnt[i];
-    n_list = (uint32_t)cta_sum(c, s.red);
+      if (MINE * tid + i <= last) c += MINE * tid + i >= first ? (u64)cnt[i] : (u64)cnt[i] << 32;
+    c = cta_sum(c, s.red);
+    n_list = (uint32_t)c;
+    n_before = (uint32_t)(c >> 32);
   }
   if (n_list <= WINDOW) {
     if (tid == 0) {
@@ -686,7 +688,34 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
       else weights<true, false, false>(row, s, weigh, f_first, f_last, least, whole, sure);
     }
     __syncthreads();
-    if (first <= last) {
+    if (first <= last && n_list <= TH) {                               // a token a thread: in order, with the weight before it
+      constexpr int SORTED = WINDOW / 2;
+      const u64 mine = tid < n_list ? s.wc[tid] : 0;
+      if (warp * 32 < n_list) {
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n_list; ++j) rank += s.wc[j] > mine;
+        if (tid < n_list) {
+          s.wc[SORTED + rank] = mine;
+          s.ww[SORTED + rank] = s.ww[tid];
+        }
+      }
+      __syncthreads();
+      const u64 c = tid < n_list ? s.wc[SORTED + tid] : 0, w = tid < n_list ? s.ww[SORTED + tid] : 0;
+      u64 all;
+      const u64 after = cta_scan<u64>(w, s.red, all), before = after - w;
+      const uint32_t limit = k_on ? min(n_list, (uint32_t)k - n_before) : n_list;
+      if (tid + 1 == limit) s.u0 = after;
+      double want = INFINITY;
+      if (p_on) {
+        sure = cta_sum(sure, s.red);
+        whole = k_on ? sure + s.u0 : cta_sum(whole, s.red);            // with top-k, its sum counts what that keeps
+        want = fmax((double)tp * (double)whole, 0.5) - (double)sure;
+      }
+      const bool keep = tid < limit && (double)before < want, next = tid + 1 < limit && (double)after < want;
+      if (keep && w >= least) atomicAdd(&s.cw[(0xffffffffu - (uint32_t)c) / (32 * PER)], w);
+      if (keep && !next) s.u1 = c;
+      if (tid == 0 && !keep) s.u1 = c + 1;
+    } else if (first <= last) {
       const uint32_t n = s.n;
       u64 floor = 0;
       if (k_on) {

@@ -185,7 +185,7 @@ def acc_rope_cache8(acc, dtype, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_sca
         return out
     dev = _check_device("acc_rope_cache8", acc, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale)
     _check_tables(cos_t, sin_t, hd)
-    out = torch.empty((T, W), dtype=dtype, device=acc.device)
+    out = acc.new_empty((T, W), dtype=dtype)
     f = _fn("dlti_acc_rope_cache8", (_V, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V))
     _lib.check(f(acc.data_ptr(), out.data_ptr(), W, pos.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), slots.data_ptr(), k8.data_ptr(), v8.data_ptr(),
                  k_scale.data_ptr(), v_scale.data_ptr(), T, H, KV, hd, bs, _lib.dtype_code(dtype), _stream(dev)), "acc_rope_cache8")
@@ -246,7 +246,7 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
         raise ValueError("paged_decode8: rows begin at multiples of 16 bytes")
     bs, width = k8.shape[2], block_tables.shape[1]
     if out is None:
-        out = torch.empty((B, H * hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((B, H * hd))
     else:
         _check_device("paged_decode8", out)
     splits = splits8(B * KV * -(-(H // KV) // 8), width * bs if max_ctx is None else min(width * bs, max_ctx))

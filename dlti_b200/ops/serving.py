@@ -291,8 +291,8 @@ def sample_given(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
         if t is not None and t.get_device() != d:
             raise ValueError(f"sample_given: every tensor is on the current device, cuda:{d}")
     if out is None:
-        out = torch.empty(B, dtype=torch.int64, device=logits.device)
-    lp = torch.empty(B, dtype=torch.float32, device=logits.device) if want_logprob else None
+        out = logits.new_empty(B, dtype=torch.int64)
+    lp = logits.new_empty(B, dtype=torch.float32) if want_logprob else None
     f = _lib.fn("dlti_sample_given", _GIVEN)
     p = [None if t is None else t.data_ptr() for t in (temperature, top_k, top_p, min_p, lp)]
     _lib.check(f(logits.data_ptr(), ld, B, V, u.data_ptr(), p[0], p[1], p[2], p[3], out.data_ptr(), p[4], _lib.dtype_code(logits.dtype),
