@@ -7,6 +7,7 @@
 #include "common.cuh"
 
 #include <cstdio>
+#include <initializer_list>
 #include <type_traits>
 
 namespace {
@@ -392,8 +393,8 @@ __device__ __forceinline__ void finish(const Attend8& p, T* out, int b, int head
   }
 }
 
-// WHOLE: a tile lies in one page (block_size a multiple of 16)
-template <typename T, bool WHOLE>
+// WHOLE: a tile lies in one page (block_size a multiple of 16). CLUSTER: the context is cut into splits
+template <typename T, bool WHOLE, bool CLUSTER>
 __global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
   extern __shared__ __align__(128) unsigned char raw[];
   AttendSmem& sm = *reinterpret_cast<AttendSmem*>(raw);
@@ -628,7 +629,7 @@ __global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
   __syncthreads();
   // Splits of one context are a cluster of up to 8 CTAs that join through distributed shared memory; with more, each cluster's sum goes to the
   // workspace.
-  const uint32_t crank = cluster_rank(), csize = cluster_size();
+  const uint32_t crank = CLUSTER ? cluster_rank() : 0, csize = CLUSTER ? cluster_size() : 1;
   const int d = threadIdx.x;
   for (int h = 0; h < nh; ++h) {
     float gm = s_m[0][h], gl = 0.f, acc = 0.f;
@@ -640,14 +641,14 @@ __global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
       gl += s_l[w][h] * a;
       acc += s_o[w][h][d] * a;
     }
-    if (csize == 1) {
+    if (!CLUSTER) {
       finish(p, reinterpret_cast<T*>(p.out), b, h0 + h, d, acc, gl, gm, split);
     } else {
       s_o[0][h][d] = acc;                                   // nobody else reads column d
       if (d == 0) s_cml[h] = make_float2(gm, gl);
     }
   }
-  if (csize == 1) return;
+  if (!CLUSTER) return;
   cluster_barrier();
   for (int h = crank; h < nh; h += csize) {
     const uint32_t ml = smem_u32(&s_cml[h]), at = smem_u32(&s_o[0][h][d]);
@@ -708,12 +709,14 @@ int attend8_t(const Attend8& p, int batch, cudaStream_t st) {
   int dev = 0;
   DLTI_CUDA_CHECK(cudaGetDevice(&dev));
   if (!set[dev & 63]) {
-    DLTI_CUDA_CHECK(cudaFuncSetAttribute(attend8_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(AttendSmem)));
-    DLTI_CUDA_CHECK(cudaFuncSetAttribute(attend8_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(AttendSmem)));
+    for (auto k : {attend8_kernel<T, true, true>, attend8_kernel<T, false, true>, attend8_kernel<T, true, false>, attend8_kernel<T, false, false>})
+      DLTI_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(AttendSmem)));
     set[dev & 63] = true;
   }
-  DLTI_CUDA_CHECK(dlti_launch_pdl_cluster(batch, p.splits / p.parts, whole ? attend8_kernel<T, true> : attend8_kernel<T, false>,
-                                          dim3(p.splits, p.KV * ((p.G + 7) / 8), batch), dim3(32 * NW), sizeof(AttendSmem), st, p));
+  const auto kernel = p.splits > 1 ? (whole ? attend8_kernel<T, true, true> : attend8_kernel<T, false, true>)
+                                   : (whole ? attend8_kernel<T, true, false> : attend8_kernel<T, false, false>);
+  DLTI_CUDA_CHECK(dlti_launch_pdl_cluster(batch, p.splits / p.parts, kernel, dim3(p.splits, p.KV * ((p.G + 7) / 8), batch),
+                                          dim3(32 * NW), sizeof(AttendSmem), st, p));
   if (p.parts > 1)
     DLTI_CUDA_CHECK(dlti_launch_pdl(batch, join8_kernel<T>, dim3(H, batch), dim3(HD), 0, st, (const float*)p.part_o, (const float*)p.part_ml,
                                     p.parts, (T*)p.out, p.out_ld));

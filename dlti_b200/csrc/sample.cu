@@ -132,7 +132,7 @@ struct Weigh {
   float top, per_bin;
   double top64, c;
   __device__ __forceinline__ Weigh(float top_, float t)
-      : top(top_), per_bin((float)NB / (RANGE * t)), top64(wide(top_)), c(1.4426950408889634074 / (double)t) {}
+      : top(top_), per_bin(fmaxf((float)NB / RANGE / t, 1e-44f)) /* of an infinite T: any but -inf is near */, top64(wide(top_)), c(1.4426950408889634074 / (double)t) {}
   // x in double by its bits (a conversion runs at a quarter of the rate): numbers below 2^-126 become others of that size, infinity 2^128
   static __device__ __forceinline__ double wide(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -590,8 +590,8 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
   __syncthreads();
 
   // a kept token weighs at least `least`
-  const double least_w = min_p ? ceil(fmax(fmin((double)min_p[b], 1.0), 0.0) * UNIT) : 0.0;
-  const u64 least = (u64)least_w;
+  const float mp = min_p ? min_p[b] : 0.f;
+  const u64 least = mp > 0.f ? (u64)ceil(fmin((double)mp, 1.0) * UNIT) : 0;
   constexpr int MINE = NB / TH;                                        // bins of a thread
   uint32_t cnt[MINE];
   if (k_on || p_on) {
@@ -688,6 +688,7 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
       else weights<true, false, false>(row, s, weigh, f_first, f_last, least, whole, sure);
     }
     __syncthreads();
+    n_list = s.n;
     if (first <= last && n_list <= TH) {                               // a token a thread: in order, with the weight before it
       constexpr int SORTED = WINDOW / 2;
       const u64 mine = tid < n_list ? s.wc[tid] : 0;
@@ -716,7 +717,7 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
       if (keep && !next) s.u1 = c;
       if (tid == 0 && !keep) s.u1 = c + 1;
     } else if (first <= last) {
-      const uint32_t n = s.n;
+      const uint32_t n = n_list;
       u64 floor = 0;
       if (k_on) {
         floor = ranked<false>(s, n, by_k, 0ull, k_left, 0.0);

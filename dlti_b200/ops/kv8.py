@@ -245,6 +245,7 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
     if unit != 1 or ld % 8 or q.data_ptr() % 16:
         raise ValueError("paged_decode8: rows begin at multiples of 16 bytes")
     bs, width = k8.shape[2], block_tables.shape[1]
+    _need(width * bs < 1 << 31, "paged_decode8: contexts have 31 bits")
     if out is None:
         out = q.new_empty((B, H * hd))
     else:

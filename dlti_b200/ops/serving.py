@@ -249,12 +249,12 @@ def sample_given_ref(logits, u, temperature=None, top_k=None, top_p=None, min_p=
     k = row(top_k, 0.0)
     keep = rank < torch.where(k > 0, k, float(V))
     run = torch.cumsum(d * keep, -1)
-    p = row(top_p, 1.0).clamp_min(0.0)
+    p = row(top_p, 1.0).nan_to_num(1.0).clamp_min(0.0)
     keep = keep & ((p >= 1) | (rank <= (run < p * run[:, -1:]).sum(-1, keepdim=True)))
-    keep = keep & (d >= row(min_p, 0.0).clamp_max(1.0))
+    keep = keep & (d >= row(min_p, 0.0).nan_to_num(0.0).clamp_max(1.0))
     kept = torch.zeros_like(w).scatter_(-1, order, d * keep)
     run = torch.cumsum(kept, -1)
-    goal = torch.minimum(u.double()[:, None].clamp_min(0.0) * run[:, -1:], run[:, -1:] * (1 - 2.3e-16))
+    goal = torch.minimum(u.double()[:, None].nan_to_num(0.0, 1.0).clamp_min(0.0) * run[:, -1:], run[:, -1:] * (1 - 2.3e-16))
     token = torch.where(drawn, ((run > goal) & (kept > 0)).long().argmax(-1), first)
     lp = (x.gather(-1, token[:, None]) - top)[:, 0].nan_to_num(0.0) - torch.where(x == top, 1.0, torch.exp(x - top).nan_to_num(0.0)).sum(-1).log()
     none = top[:, 0] == float("-inf")
@@ -268,7 +268,7 @@ def sample_given(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
     Weights are exp((x - max) / temperature). Of the tokens by descending logit, ties by ascending index, the first top_k are kept; of these the
     fewest that hold top_p of their weight; of these the ones of at least min_p times the largest weight. The draw is the first token, by index, at
     which the running sum of what is kept exceeds u times its sum. Temperature <= 0: the largest logit at its lowest index. NaN counts as -inf; a
-    row of nothing else gives token 0 and log-prob -inf. The same logits and numbers give the same tokens everywhere."""
+    row of nothing else gives token 0 and log-prob -inf. A setting that is NaN is off. The same logits and numbers give the same tokens everywhere."""
     B, V = logits.shape
     if u.dtype is not torch.float64 or u.shape != (B,) or not u.is_contiguous():
         raise ValueError("sample_given: a float64 number for each row")

@@ -196,14 +196,13 @@ class LLMEngine:
             raise ValueError(f"{cfg.name}: pages in 8 bits are available for the Llama family only")
         if fork_samples and self.world > 1:
             raise ValueError("fork_samples copies pages on one GPU only")
+        if fork_samples and self.per_sequence:
+            raise ValueError(f"{cfg.name}: fork_samples is available for the Llama family only")
         self.slots = None
         if any(s is not None for s in state_specs):
             if enable_prefix_caching:
                 raise ValueError(f"{cfg.name}: prefix caching shares pages of keys and values, but this model also carries "
                                  "recurrent state from token to token")
-            if fork_samples:
-                raise ValueError(f"{cfg.name}: fork_samples shares pages of keys and values, but this model also carries recurrent state "
-                                 "from token to token")
             self.slots = SlotManager(max_num_seqs)
             self.states = StateCache(state_specs, max_num_seqs, self.dtype, self.device)
         else:

@@ -82,6 +82,7 @@ def attend_error(out, mag, reach, ctx, dtype, hd):
 
 def token(x, u, t, top_k, top_p, min_p):
     """One row: the token by the definition, in plain Python floats (math.fsum for every sum)."""
+    top_p, min_p, u = (off if math.isnan(v) else v for v, off in ((top_p, 1.0), (min_p, 0.0), (u, 0.0)))
     x = [float("-inf") if math.isnan(v) else float(v) for v in x]
     top = max(x)
     if top == float("-inf"):

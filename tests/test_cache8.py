@@ -337,6 +337,91 @@ def test_gather(dev, dtype, n, H, KV, bs):
     assert got.data_ptr() == e.data_ptr() and torch.equal(got.cpu(), want)
 
 
+# ---- as programs call them ----------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_far_pages():
+    """Caches of more than 2^31 bytes: rows written to their last pages, read back and attended to, as near the begin of a small one."""
+    n, KV, bs = (1 << 20) + 700, 1, 16
+    far = [n - 1, n - 300, n - 2, (1 << 20) + 1, 5]
+    big = [torch.zeros((n, KV, bs, HD), dtype=torch.uint8, device="cuda").view(E4) for _ in range(2)]
+    small = [torch.zeros((5, KV, bs, HD), dtype=torch.uint8, device="cuda").view(E4) for _ in range(2)]
+    cos, sin = rope_tables(80, HD, 10000.0, "cuda")
+    x = torch.randn((70, 4 * HD), generator=gen(1)).to(torch.bfloat16).cuda()
+    got = []
+    for (k, v), pages_ in ((big, far), (small, [0, 1, 2, 3, 4])):
+        ks, vs = (torch.full(k.shape[:2], 2.0 ** -120, device="cuda") for _ in range(2))
+        slots = torch.tensor([pages_[j // bs] * bs + j % bs for j in range(70)], device="cuda")
+        rows = kv8.rope_cache8_(x.clone(), torch.arange(70, dtype=torch.int32, device="cuda"), cos, sin, slots, k, v, ks, vs, 2, KV, HD)
+        ext = torch.zeros_like(rows)
+        kv8.gather_rows8_(ext, torch.arange(70, device="cuda"), slots, k, v, ks, vs, 2, KV, HD)
+        t = torch.tensor([pages_], dtype=torch.int32, device="cuda")
+        o = kv8.paged_decode8(rows[-1:], k, v, ks, vs, t, torch.tensor([70], dtype=torch.int32, device="cuda"), 2, KV, HD)
+        got.append((rows, ext, o))
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and float(got[0][2].abs().sum()) > 0
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("bs", [8, 16, 24])
+def test_table_entries_behind_the_context(dev, bs):
+    """They are not read: any number may stand there."""
+    def edit(q, k8, v8, ks, vs, table):
+        for i, n in enumerate((3 * bs, 2 * bs + 5, 0, 1)):
+            table[i, -(-n // bs):] = 1 << 30
+    check_attend([3 * bs, 2 * bs + 5, 0, 1], 4, 2, bs, torch.bfloat16, dev, seed=1, edit=edit, wide=9, max_ctx=5000)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reach", [64, 700, 60000])
+def test_streams_and_graphs(reach):
+    """A decode step (rows, attention) on a stream of its own, and captured twice: the graphs share nothing but the cache, are replayed side by side
+    on two streams, and follow what their buffers hold."""
+    KV, H, bs, B = 2, 8, 16, 3
+    width = max(4, reach // bs)
+    n = 3 * 50 + 1
+    cache = (*pages(n, KV, bs, 1, 1, "cuda"), *pages(n, KV, bs, 2, 1, "cuda"))
+    k8, ks, v8, vs = cache
+    table = torch.zeros((B, width), dtype=torch.int32)
+    for b in range(B):
+        table[b, :min(width, 50)] = torch.arange(50)[:width] + 50 * b
+    table = table.cuda()
+    cos, sin = rope_tables(900, HD, 10000.0, "cuda")
+    lens = torch.tensor([5, 60, 33], dtype=torch.int32, device="cuda")
+    x = torch.randn((B, (H + 2 * KV) * HD), generator=gen(3)).to(torch.bfloat16).cuda()
+
+    slots = torch.tensor([int(table[b, (m - 1) // bs]) * bs + (m - 1) % bs for b, m in enumerate(lens.tolist())], device="cuda")
+
+    def step(x, kk, kss, vv, vss):
+        rows = kv8.rope_cache8_(x, lens - 1, cos, sin, slots, kk, vv, kss, vss, H, KV, HD, out=torch.empty_like(x))
+        return kv8.paged_decode8(rows, kk, vv, kss, vss, table, lens, H, KV, HD, max_ctx=reach)
+
+    fresh = lambda: tuple(t.clone() for t in cache)
+    want = [step(y, *fresh()).clone() for y in (x, x * 2)]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    mine = fresh()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        got = step(x, *mine)
+    s.synchronize()
+    assert torch.equal(got, want[0])
+    sets = []
+    for _ in range(2):
+        y, c = x.clone(), fresh()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = step(y, *c)
+        sets.append((g, y, o))
+    sets[1][1].copy_(x * 2)
+    torch.cuda.synchronize()
+    for (g, _, _), stream in zip(sets, (s, torch.cuda.Stream())):
+        with torch.cuda.stream(stream):
+            for _ in range(3):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(sets[0][2], want[0]) and torch.equal(sets[1][2], want[1])
+
+
 # ---- refusals -------------------------------------------------------------------------------------------------------------------
 def test_refusals():
     k8, ks = pages(4, 2, 16, 1)

@@ -148,6 +148,60 @@ def test_pitch_alignment_and_out(dev):
         assert want.tolist() == [R.token(r, v, 1.0, 40, 1.0, 0.0) for r, v in zip(x.cpu().double().tolist(), u.cpu().tolist())]
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_settings_that_are_no_numbers(dev):
+    """A temperature that is NaN is greedy, any other setting that is NaN is off, a number that is NaN draws as 0; an infinite temperature is flat."""
+    x, u = logits(5, 900, 2), uniform(5, 3)
+    x[4, 100:] = -math.inf
+    nan = math.nan
+    run(x, u, [nan, 1.0, 1.0, 1.0, math.inf], [0, 20, 0, 0, 500], [0.9, nan, 0.9, 1.0, 1.0], [0.0, 0.0, nan, nan, 0.0], dev)
+    v = u.clone()
+    v[1] = nan
+    t = torch.ones(5, device=dev)
+    a, _ = S.sample_given(x.to(dev), v.to(dev), t)
+    b, _ = S.sample_given(x.to(dev), v.nan_to_num(0.0).to(dev), t)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_cuts_that_need_more_than_the_list(dev):
+    """Logits in groups of many equal ones, at every distance: cuts inside a group, top-k and top-p in different groups, long lists and short ones."""
+    V, g = 18000, torch.Generator().manual_seed(1)
+    levels = torch.tensor([3.0, 2.99, 2.5, 2.0, 0.0, -1.0, -9.0, -40.0])
+    x = levels[torch.multinomial(torch.tensor([0.002, 0.01, 0.05, 0.3, 0.3, 0.2, 0.1, 0.038]), V, replacement=True, generator=g)].expand(12, V).clone()
+    k = [0, 0, 0, 100, 1500, 7000, 9000, 17900, 3000, 12000, 30, 5]
+    p = [0.5, 0.9, 0.999, 1.0, 1.0, 1.0, 0.7, 0.5, 0.9, 0.3, 0.2, 0.999]
+    for dtype in (torch.float32, torch.float16):
+        for t in (1.0, 0.3, 4.0):
+            run(x.to(dtype), uniform(12, 7), t, k, p, [0.0, 0.0, 0.02] * 4, dev)
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    """On a stream of its own, and captured: replays follow what the buffers hold."""
+    x, u = logits(6, 5000, 5).cuda(), uniform(6, 6).cuda()
+    t, k, p = torch.ones(6, device="cuda"), torch.full((6,), 300, dtype=torch.int32, device="cuda"), torch.full((6,), 0.9, device="cuda")
+    want = [S.sample_given(y, u, t, k, p)[0].tolist() for y in (x, x.flip(0))]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        a, _ = S.sample_given(x, u, t, k, p)
+    s.synchronize()
+    assert a.tolist() == want[0]
+    y = x.clone()
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            o, _ = S.sample_given(y, u, t, k, p)
+        graphs.append((gr, o))
+    y.copy_(x.flip(0))
+    for gr, _ in graphs:
+        gr.replay()
+    torch.cuda.synchronize()
+    assert [o.tolist() for _, o in graphs] == [want[1]] * 2
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("V", [131072, 262144])
 def test_long_rows(V):
