@@ -25,6 +25,9 @@ constexpr int TH = 512, WARPS = TH / 32, PER = 8; // threads, and consecutive to
 constexpr int CHUNK = TH * PER;
 constexpr int NB = 8192, ND = 2048;               // bins of the distance from the largest; digits of 11 bits
 constexpr int LIST = 512, WINDOW = 7168;
+// Half of the range that is looked at first, relative to top-p's sum. The mean of a bin's bounds is off by at most 2^-9 of a token's weight, evenly
+// to either side: by 3e-5 of the sum of a thousand tokens of one weight.
+constexpr float NEAR = 3e-4f;
 constexpr int V_MAX = 1 << 18, GROUPS = V_MAX / (32 * PER);
 constexpr double UNIT = 35184372088832.0;         // 2^45
 constexpr float RANGE = 32.f;                     // bins reach this far below the largest logit, in units of T: e^-32 < 2^-46
@@ -45,7 +48,7 @@ struct Work {
   u64 red[32];
   float fred[32];
   u64 u0, u1;
-  int i0, i1;
+  int i0, i1, g0, g1;
   uint32_t n;
 };
 
@@ -471,23 +474,47 @@ __device__ __noinline__ void weights(const Row<T> row, Work& s, const Weigh weig
   u64 whole = 0, sure = 0;
   row.each_chunk([&](int c, int base, const float (&x)[PER]) {
     u64 kept = 0;
+    auto count = [&](u64 w, float at) {
+      const u64 before = at < f_first ? w : 0;
+      if (SUM) whole += w;
+      if (CUT) {
+        sure += before;
+        kept += before >= least ? before : 0;
+      } else {
+        kept += before;
+      }
+    };
+    auto list = [&](u64 w, float at, int j) {
+      if (at >= f_first && at < f_last && base + j < row.V) {
+        const uint32_t i = atomicAdd(&s.n, 1u);
+        s.wc[i] = place(x[j], base + j);
+        s.ww[i] = w;
+      }
+    };
+    if constexpr (EVERY) {                                             // nothing in between: eight chains of operations side by side
+      u64 w[PER];
+      float at[PER];
+      bool near = false;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {                                    // those behind the end are -inf: no weight
-      const float at = below(weigh.top, x[j]) * weigh.per_bin;
-      if (EVERY || __any_sync(0xffffffffu, at < f_last)) {
-        const u64 w = EVERY || at < f_last ? weigh(x[j], at) : 0;
-        const u64 before = at < f_first ? w : 0;
-        if (SUM) whole += w;
-        if (CUT) {
-          sure += before;
-          kept += before >= least ? before : 0;
-        } else {
-          kept += before;
-        }
-        if (at >= f_first && at < f_last && base + j < row.V) {
-          const uint32_t i = atomicAdd(&s.n, 1u);
-          s.wc[i] = place(x[j], base + j);
-          s.ww[i] = w;
+      for (int j = 0; j < PER; ++j) {                                  // those behind the end are -inf: no weight
+        at[j] = below(weigh.top, x[j]) * weigh.per_bin;
+        near |= at[j] >= f_first && at[j] < f_last;
+        w[j] = weigh(x[j], at[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < PER; ++j) count(w[j], at[j]);
+      if (near) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) list(w[j], at[j], j);
+      }
+    } else {                                                           // few count: most warps see none
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const float at = below(weigh.top, x[j]) * weigh.per_bin;
+        if (__any_sync(0xffffffffu, at < f_last)) {
+          const u64 w = at < f_last ? weigh(x[j], at) : 0;
+          count(w, at);
+          list(w, at, j);
         }
       }
     }
@@ -618,7 +645,7 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
     k_left = (uint32_t)k - (uint32_t)s.u0;
     __syncthreads();
   }
-  int from = NB, to = -1;                                              // bins in which top-p can end
+  int from = NB, to = -1, near_from = NB, near_to = -1;                // bins in which top-p can end, and does most of the time
   if (p_on) {
     // a bin's weight lies between its count times its least and its largest weight; so do the running sums, and with them the bins in which the
     // sum can reach top_p of the whole
@@ -639,37 +666,66 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
     float al = cta_scan<float>(ls, s.fred, lowest) - ls;
     const float pp = fmaxf(tp, 0.f);
     const float lo_goal = pp * lowest * 0.9999f, hi_goal = pp * most * 1.0001f;
-    if (tid == 0) s.i0 = s.i1 = k_bin;
+    // The mean of both bounds is far nearer (a bin's tokens lie evenly in it): where the bounds leave many tokens, a narrow range around it is
+    // looked at first, and the weights themselves tell whether top-p ends there.
+    const float mid_goal = pp * 0.5f * (most + lowest);
+    if (tid == 0) {
+      s.i0 = s.i1 = k_bin;
+      s.g0 = s.g1 = k_bin;
+    }
     __syncthreads();
-    bool h_done = false, l_done = false;
+    // only threads near where a goal is reached look for it (all those behind it would queue for the same word)
+    const float mid0 = 0.5f * (ah + al);
+    bool h_done = ah > lo_goal * 1.0001f, l_done = al > hi_goal * 1.0001f, a_done = mid0 > mid_goal, b_done = mid0 > mid_goal * 1.001f;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
       ah += hi[i];
       al += lo[i];
       if (!h_done && ah >= lo_goal) { atomicMin(&s.i0, MINE * tid + i); h_done = true; }
       if (!l_done && al >= hi_goal) { atomicMin(&s.i1, MINE * tid + i); l_done = true; }
+      const float mid = 0.5f * (ah + al);
+      if (!a_done && mid >= mid_goal * (1.f - NEAR)) { atomicMin(&s.g0, MINE * tid + i); a_done = true; }
+      if (!b_done && mid >= mid_goal * (1.f + NEAR)) { atomicMin(&s.g1, MINE * tid + i); b_done = true; }
     }
     __syncthreads();
     from = s.i0;
     to = max(s.i1, from);
+    near_from = min(max(from, s.g0), to);
+    near_to = min(to, max(s.g1, near_from));
     __syncthreads();
   }
   // bins first .. last are looked at token by token; those before are kept, those behind are not (but count for top-p's sum, without top-k)
-  const int first = p_on ? from : k_on ? k_bin : NB, last = k_on ? k_bin : to;
   const Group by_k{top, per_bin, 0, 0, k_bin};
   Group by_p{top, per_bin, from, 0, 0};
   while (((to - from) >> by_p.shift) >= ND) ++by_p.shift;
-  uint32_t n_list = 0, n_before = 0;                                   // their tokens, and those before them
+  int first = p_on ? from : k_on ? k_bin : NB, last = k_on ? k_bin : to;
+  uint32_t n_list = 0, n_before = 0;                                   // their tokens, and those before them (with top-k; else those of the near bins)
   if (first <= last) {
     u64 c = 0;
 #pragma unroll
-    for (int i = 0; i < MINE; ++i)
-      if (MINE * tid + i <= last) c += MINE * tid + i >= first ? (u64)cnt[i] : (u64)cnt[i] << 32;
+    for (int i = 0; i < MINE; ++i) {
+      const int at = MINE * tid + i;
+      if (at <= last && at >= first) c += cnt[i];
+      if (k_on ? at < first : at >= near_from && at <= near_to) c += (u64)cnt[i] << 32;
+    }
     c = cta_sum(c, s.red);
     n_list = (uint32_t)c;
     n_before = (uint32_t)(c >> 32);
   }
-  if (n_list <= WINDOW) {
+  const bool guess = !k_on && n_list > TH;
+  if (guess) {
+    first = near_from;
+    last = near_to;
+    n_list = n_before;
+  }
+  Group near = by_p;
+  if (guess) {
+    near.base = near_from;
+    near.shift = 0;
+    while (((near_to - near_from) >> near.shift) >= ND) ++near.shift;
+  }
+  bool again = n_list > WINDOW;
+  if (!again) {
     if (tid == 0) {
       s.n = 0;
       s.u0 = 0;
@@ -712,10 +768,13 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
         whole = k_on ? sure + s.u0 : cta_sum(whole, s.red);            // with top-k, its sum counts what that keeps
         want = fmax((double)tp * (double)whole, 0.5) - (double)sure;
       }
-      const bool keep = tid < limit && (double)before < want, next = tid + 1 < limit && (double)after < want;
-      if (keep && w >= least) atomicAdd(&s.cw[(0xffffffffu - (uint32_t)c) / (32 * PER)], w);
-      if (keep && !next) s.u1 = c;
-      if (tid == 0 && !keep) s.u1 = c + 1;
+      again = guess && !(want > 0.0 && want <= (double)s.u0);
+      if (!again) {
+        const bool keep = tid < limit && (double)before < want, next = tid + 1 < limit && (double)after < want;
+        if (keep && w >= least) atomicAdd(&s.cw[(0xffffffffu - (uint32_t)c) / (32 * PER)], w);
+        if (keep && !next) s.u1 = c;
+        if (tid == 0 && !keep) s.u1 = c + 1;
+      }
     } else if (first <= last) {
       const uint32_t n = n_list;
       u64 floor = 0;
@@ -735,21 +794,27 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
         __syncthreads();
         for (uint32_t i = tid; i < n; i += TH)
           if (s.wc[i] >= floor) {
-            const int g = by_p.of(logit_of(s.wc[i]));
+            const int g = near.of(logit_of(s.wc[i]));
             if (g < ND) atomicAdd(&s.mass[g], s.ww[i]);
           }
         __syncthreads();
         double want = fmax((double)tp * (double)whole, 0.5) - (double)sure;
-        by_p.g = reached(s, want);
-        if (by_p.g >= 0) floor = ranked<true>(s, n, by_p, floor, 0u, want);      // else nothing is cut
+        again = guess && want <= 0.0;
+        near.g = reached(s, want);
+        again |= guess && near.g < 0;
+        if (!again && near.g >= 0) floor = ranked<true>(s, n, near, floor, 0u, want);       // else nothing is cut
       }
-      for (uint32_t i = tid; i < n; i += TH)
-        if (s.wc[i] >= floor && s.ww[i] >= least) atomicAdd(&s.cw[(0xffffffffu - (uint32_t)s.wc[i]) / (32 * PER)], s.ww[i]);
-      if (tid == 0) s.u1 = floor;
+      if (!again) {
+        for (uint32_t i = tid; i < n; i += TH)
+          if (s.wc[i] >= floor && s.ww[i] >= least) atomicAdd(&s.cw[(0xffffffffu - (uint32_t)s.wc[i]) / (32 * PER)], s.ww[i]);
+        if (tid == 0) s.u1 = floor;
+      }
     } else if (tid == 0) {
       s.u1 = 0;
     }
-  } else {
+    __syncthreads();
+  }
+  if (again) {
     const u64 floor = cut_by_division(row, s, weigh, k_on, by_k, k_left, p_on, by_p, to, tp);
     for (int c = 0; c < chunks; ++c) {
       const int base = c * CHUNK + tid * PER;
