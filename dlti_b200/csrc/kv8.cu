@@ -73,7 +73,7 @@ struct Rows8 {
   const long long* slots;
   uint8_t *k8, *v8;
   float *ks, *vs;
-  int tokens, H, KV, bs;
+  int tokens, H, KV, bs, shift;  // shift: bs = 1 << shift, or -1
 };
 
 template <typename T, bool ACC>
@@ -97,33 +97,54 @@ struct RowsCfg {
 using DecodeRows = RowsCfg<1, 1, 4>;
 using PromptRows = RowsCfg<16, 8, 3>;
 
-// cosines and sines of row t in the rows' type, rounded as the 16-bit cache's ops round them
-template <typename T>
+// cosines and sines of a row, rounded to the rows' type as the 16-bit cache's ops round them
 struct Angles {
-  int4 c, s;
+  float c[8], s[8];
 };
 template <typename T>
-__device__ __forceinline__ int4 rounded8(const float* f) {
-  const float4 a = *reinterpret_cast<const float4*>(f), b = *reinterpret_cast<const float4*>(f + 4);
-  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  return pack8<T>(v);
+__device__ __forceinline__ float4 rounded4(const float* f) {
+  const float4 a = *reinterpret_cast<const float4*>(f);
+  return make_float4(Cvt<T>::to_f(Cvt<T>::from_f(a.x)), Cvt<T>::to_f(Cvt<T>::from_f(a.y)), Cvt<T>::to_f(Cvt<T>::from_f(a.z)), Cvt<T>::to_f(Cvt<T>::from_f(a.w)));
+}
+// the larger of a pair and the magnitudes of eight elements; NaN is passed over
+template <typename T>
+__device__ __forceinline__ uint32_t larger(uint32_t top, const int4& v);
+template <>
+__device__ __forceinline__ uint32_t larger<__nv_bfloat16>(uint32_t top, const int4& v) {
+  const uint32_t u[4] = {(uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = u[i] & 0x7fff7fffu;
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&top), *reinterpret_cast<const __nv_bfloat162*>(&a));
+    top = *reinterpret_cast<const uint32_t*>(&m);
+  }
+  return top;
+}
+template <>
+__device__ __forceinline__ uint32_t larger<__half>(uint32_t top, const int4& v) {
+  const uint32_t u[4] = {(uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = u[i] & 0x7fff7fffu;
+    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&top), *reinterpret_cast<const __half2*>(&a));
+    top = *reinterpret_cast<const uint32_t*>(&m);
+  }
+  return top;
 }
 // The lane's 8 elements rotated (all lanes of the warp call). Products of two 16-bit numbers are exact in fp32, so one rounding is left.
 template <typename T>
-__device__ __forceinline__ int4 turn(const int4& v, const Angles<T>& an, bool low) {
+__device__ __forceinline__ int4 turn(const int4& v, const Angles& an, bool low) {
   int4 w;
   w.x = __shfl_xor_sync(0xffffffffu, v.x, 8);
   w.y = __shfl_xor_sync(0xffffffffu, v.y, 8);
   w.z = __shfl_xor_sync(0xffffffffu, v.z, 8);
   w.w = __shfl_xor_sync(0xffffffffu, v.w, 8);
   if (low) w = make_int4(w.x ^ 0x80008000, w.y ^ 0x80008000, w.z ^ 0x80008000, w.w ^ 0x80008000);
-  float a[8], b[8], c[8], s[8];
+  float a[8], b[8];
   unpack8<T>(v, a);
   unpack8<T>(w, b);
-  unpack8<T>(an.c, c);
-  unpack8<T>(an.s, s);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] = a[j] * c[j] + b[j] * s[j];
+  for (int j = 0; j < 8; ++j) a[j] = a[j] * an.c[j] + b[j] * an.s[j];
   return pack8<T>(a);
 }
 
@@ -131,44 +152,44 @@ template <typename T, bool ACC, typename C>
 __global__ void __launch_bounds__(256, C::CTAS) rows8_kernel(const Rows8 p) {
   constexpr int block = C::ROWS, KEEP = C::KEEP, STAGED = block == 1 ? 1 : 2 * block;
   griddep_pass(p.tokens);
-  __shared__ int4 s_angle[STAGED][16];                    // of a row: 8 pieces of cosines, 8 of sines
+  __shared__ float4 s_angle[STAGED][32];                    // of a row: 16 pieces of cosines, 16 of sines
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l16 = lane & 15, half = lane >> 4;
   const int first = blockIdx.x * block, last = min(p.tokens, first + block);
   const int staged = min(p.tokens - first, STAGED);
   const bool copy = ACC || p.out != p.x, low = l16 < 8;
   T* out = reinterpret_cast<T*>(p.out);
-  for (int i = threadIdx.x; i < staged * 16; i += 256) {
-    const long long at = (long long)p.pos[first + (i >> 4)] * (HD / 2) + (i & 7) * 8;
-    s_angle[i >> 4][i & 15] = rounded8<T>((i & 8 ? p.sin_t : p.cos_t) + at);
+  const int heads = p.H + 2 * p.KV;
+  int4 held[KEEP];
+  // rows t, t + 1, ... of a run of n
+  auto request = [&](int t, int n, int col) {
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      held[i] = make_int4(0, 0, 0, 0);
+      if (2 * i + half < n) held[i] = take<T, ACC>(p, t + 2 * i + half, col, l16);
+    }
+  };
+  for (int i = threadIdx.x; i < staged * 32; i += 256) {
+    const long long at = (long long)p.pos[first + (i >> 5)] * (HD / 2) + (i & 15) * 4;
+    s_angle[i >> 5][i & 31] = rounded4<T>((i & 16 ? p.sin_t : p.cos_t) + at);
   }
   __syncthreads();
   auto angles = [&](int t) {
-    Angles<T> a;
+    const int q = (l16 & 7) * 2;
+    float4 c0, c1, s0, s1;
     if (t - first < staged) {
-      a.c = s_angle[t - first][l16 & 7];
-      a.s = s_angle[t - first][8 + (l16 & 7)];
+      const float4* a = s_angle[t - first];
+      c0 = a[q], c1 = a[q + 1], s0 = a[16 + q], s1 = a[17 + q];
     } else {
-      const long long at = (long long)p.pos[t] * (HD / 2) + (l16 & 7) * 8;
-      a.c = rounded8<T>(p.cos_t + at);
-      a.s = rounded8<T>(p.sin_t + at);
+      const long long at = (long long)p.pos[t] * (HD / 2) + q * 4;
+      c0 = rounded4<T>(p.cos_t + at), c1 = rounded4<T>(p.cos_t + at + 4), s0 = rounded4<T>(p.sin_t + at), s1 = rounded4<T>(p.sin_t + at + 4);
     }
-    return a;
+    return Angles{{c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w}};
   };
   auto put_out = [&](int t, int col, const int4& v) { *reinterpret_cast<int4*>(out + t * p.out_ld + col * HD + l16 * 8) = v; };
-  const int heads = p.H + 2 * p.KV;
   for (int col = blockIdx.y * 8 + warp; col < heads; col += gridDim.y * 8) {
-    int4 held[KEEP];
-    // rows t + 16 k ... of a run of n
-    auto request = [&](int t, int n) {
-#pragma unroll
-      for (int i = 0; i < KEEP; ++i) {
-        held[i] = make_int4(0, 0, 0, 0);
-        if (2 * i + half < n) held[i] = take<T, ACC>(p, t + 2 * i + half, col, l16);
-      }
-    };
     if (col < p.H) {                                        // a query head
       for (int at = first; at < last; at += 2 * KEEP) {
-        request(at, last - at);
+        request(at, last - at, col);
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) {
           const int t = at + 2 * i + half;
@@ -185,7 +206,8 @@ __global__ void __launch_bounds__(256, C::CTAS) rows8_kernel(const Rows8 p) {
     uint8_t* cache = key ? p.k8 : p.v8;
     float* scales = key ? p.ks : p.vs;
     const uint32_t bs = p.bs;
-    auto page_of = [&](int t) { const long long s = p.slots[t]; return s < 0 ? -1 : (int)((uint32_t)s / bs); };
+    auto page_in = [&](long long s) { return p.shift >= 0 ? (int)((uint32_t)s >> p.shift) : (int)((uint32_t)s / bs); };
+    auto page_of = [&](int t) { const long long s = p.slots[t]; return s < 0 ? -1 : page_in(s); };
     for (int t = first; t < last;) {
       const int page = page_of(t);
       if (page >= 0 && t == first && t > 0 && page_of(t - 1) == page) {   // these rows belong to the block before
@@ -200,7 +222,7 @@ __global__ void __launch_bounds__(256, C::CTAS) rows8_kernel(const Rows8 p) {
         for (int k = 0;; k += 32) {
           const int r = t + k + lane;
           const long long s = r < p.tokens ? p.slots[r] : -1;
-          const bool in = s >= 0 && (int)((uint32_t)s / bs) == page;
+          const bool in = s >= 0 && page_in(s) == page;
           const uint32_t place = (uint32_t)s - (uint32_t)page * bs;
           if (k == 0) off = place;
           const uint32_t out_of = ~__ballot_sync(0xffffffffu, in);
@@ -214,26 +236,43 @@ __global__ void __launch_bounds__(256, C::CTAS) rows8_kernel(const Rows8 p) {
       float old = pow2i(E_LOW);
       if (page >= 0 && !fresh) old = scales[sc];
       float largest = 0.f;
+      uint32_t top = 0;
       for (int k = 0; k < n; k += 2 * KEEP) {
-        request(t + k, n - k);
+        request(t + k, n - k, col);
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) {
           if (k + 2 * i >= n) break;
           const int r = k + 2 * i + half;
           if (key) held[i] = turn<T>(held[i], angles(t + min(r, n - 1)), low);
           if (r < n && (key || copy)) put_out(t + r, col, held[i]);
-          float f[8];
-          unpack8<T>(held[i], f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float a = fabsf(f[j]);
-            largest = fmaxf(largest, a < INFINITY ? a : 0.f);             // neither infinities nor NaN set the scale; rows that are not there are 0
-          }
+          top = larger<T>(top, held[i]);                    // rows that are not there are 0
         }
       }
       if (page >= 0) {
+        auto of_warp = [&]() {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+          for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        };
+        const float2 pair = Cvt<T>::unpack2(top);
+        largest = fmaxf(pair.x, pair.y);
+        of_warp();
+        if (largest == INFINITY) {                          // infinities do not set the scale (nor does NaN): once more without them
+          largest = 0.f;
+          auto finite = [&](const int4& v) {
+            float f[8];
+            unpack8<T>(v, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) largest = fmaxf(largest, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
+          };
+          if (n <= 2 * KEEP) {
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i)
+              if (2 * i + half < n) finite(held[i]);
+          } else {
+            for (int r = half; r < n; r += 2) finite(*reinterpret_cast<const int4*>(out + (long long)(t + r) * p.out_ld + col * HD + l16 * 8));
+          }
+          of_warp();
+        }
         uint8_t* piece = cache + sc * bs * HD;
         const float now = fmaxf(old, scale_for(largest));
         if (!fresh && now > old) {                          // what the page holds is rounded to the new scale
@@ -781,7 +820,7 @@ DLTI_API int dlti_rope_cache8(const void* x, long long x_ld, void* out, long lon
   if (!sizes_ok("rope_cache8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
   if (tokens <= 0) return 0;
   if (tokens > 1 << 24) return DLTI_ERR_TOO_LARGE;
-  const Rows8 p{x, out, x_ld, out_ld, pos, cos_t, sin_t, slots, (uint8_t*)k8, (uint8_t*)v8, ks, vs, (int)tokens, H, KV, bs};
+  const Rows8 p{x, out, x_ld, out_ld, pos, cos_t, sin_t, slots, (uint8_t*)k8, (uint8_t*)v8, ks, vs, (int)tokens, H, KV, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs)};
   if (dtype == DLTI_BF16) return rows8_t<__nv_bfloat16, false>(p, st);
   if (dtype == DLTI_FP16) return rows8_t<__half, false>(p, st);
   return DLTI_ERR_UNSUPPORTED;
@@ -794,7 +833,7 @@ DLTI_API int dlti_acc_rope_cache8(float* acc, void* out, long long out_ld, const
   if (!sizes_ok("acc_rope_cache8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
   if (tokens <= 0) return 0;
   if (tokens > 1 << 24) return DLTI_ERR_TOO_LARGE;
-  const Rows8 p{acc, out, (long long)(H + 2 * KV) * HD, out_ld, pos, cos_t, sin_t, slots, (uint8_t*)k8, (uint8_t*)v8, ks, vs, (int)tokens, H, KV, bs};
+  const Rows8 p{acc, out, (long long)(H + 2 * KV) * HD, out_ld, pos, cos_t, sin_t, slots, (uint8_t*)k8, (uint8_t*)v8, ks, vs, (int)tokens, H, KV, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs)};
   if (dtype == DLTI_BF16) return rows8_t<__nv_bfloat16, true>(p, st);
   if (dtype == DLTI_FP16) return rows8_t<__half, true>(p, st);
   return DLTI_ERR_UNSUPPORTED;
