@@ -173,33 +173,47 @@ __global__ void __launch_bounds__(256, C::CTAS) rows8_kernel(const Rows8 p) {
     s_angle[i >> 5][i & 31] = rounded4<T>((i & 16 ? p.sin_t : p.cos_t) + at);
   }
   __syncthreads();
+  auto staged_angles = [&](int t) {
+    const float4* a = s_angle[t - first] + (l16 & 7) * 2;
+    const float4 c0 = a[0], c1 = a[1], s0 = a[16], s1 = a[17];
+    return Angles{{c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w}};
+  };
   auto angles = [&](int t) {
-    const int q = (l16 & 7) * 2;
-    float4 c0, c1, s0, s1;
-    if (t - first < staged) {
-      const float4* a = s_angle[t - first];
-      c0 = a[q], c1 = a[q + 1], s0 = a[16 + q], s1 = a[17 + q];
-    } else {
-      const long long at = (long long)p.pos[t] * (HD / 2) + q * 4;
-      c0 = rounded4<T>(p.cos_t + at), c1 = rounded4<T>(p.cos_t + at + 4), s0 = rounded4<T>(p.sin_t + at), s1 = rounded4<T>(p.sin_t + at + 4);
-    }
+    if (t - first < staged) return staged_angles(t);
+    const long long at = (long long)p.pos[t] * (HD / 2) + (l16 & 7) * 8;
+    const float4 c0 = rounded4<T>(p.cos_t + at), c1 = rounded4<T>(p.cos_t + at + 4), s0 = rounded4<T>(p.sin_t + at), s1 = rounded4<T>(p.sin_t + at + 4);
     return Angles{{c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w}};
   };
   auto put_out = [&](int t, int col, const int4& v) { *reinterpret_cast<int4*>(out + t * p.out_ld + col * HD + l16 * 8) = v; };
-  for (int col = blockIdx.y * 8 + warp; col < heads; col += gridDim.y * 8) {
-    if (col < p.H) {                                        // a query head
-      for (int at = first; at < last; at += 2 * KEEP) {
-        request(at, last - at, col);
+  const int stride = gridDim.y * 8;
+  int col = blockIdx.y * 8 + warp;
+  // query heads: the angles of two rows serve two of them (reading them for every head took 29 us of 107 MB of queries, 22 without)
+  constexpr int QH = KEEP >= 4 ? 2 : 1, QP = KEEP / QH;
+  for (; col < p.H; col += QH * stride) {
+    for (int at = first; at < last; at += 2 * QP) {
 #pragma unroll
-        for (int i = 0; i < KEEP; ++i) {
+      for (int i = 0; i < QP; ++i)
+#pragma unroll
+        for (int j = 0; j < QH; ++j) {
           const int t = at + 2 * i + half;
-          if (at + 2 * i >= last) break;
-          const int4 v = turn<T>(held[i], angles(min(t, last - 1)), low);
-          if (t < last) put_out(t, col, v);
+          held[i * QH + j] = make_int4(0, 0, 0, 0);
+          if (t < last && col + j * stride < p.H) held[i * QH + j] = take<T, ACC>(p, t, col + j * stride, l16);
         }
+#pragma unroll
+      for (int i = 0; i < QP; ++i) {
+        if (at + 2 * i >= last) break;
+        const int t = at + 2 * i + half;
+        const Angles an = staged_angles(min(t, last - 1));
+#pragma unroll
+        for (int j = 0; j < QH; ++j)
+          if (col + j * stride < p.H) {
+            const int4 v = turn<T>(held[i * QH + j], an, low);
+            if (t < last) put_out(t, col + j * stride, v);
+          }
       }
-      continue;
     }
+  }
+  for (col = p.H + (blockIdx.y * 8 + warp + stride * heads - p.H) % stride; col < heads; col += stride) {
     const int hh = col - p.H;                               // key heads, then value heads
     const bool key = hh < p.KV;
     const int head = key ? hh : hh - p.KV;
