@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
     float z[2][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};      // two chains of four products are shorter than one of eight
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int4 k = lds128(kv + (8 * h + g) * 128 + ((2 * t + i) ^ g) * 16);
@@ -582,12 +582,12 @@ __global__ void __launch_bounds__(32 * NW, 3) attend8_kernel(const Attend8 p) {
         for (int w = 0; w < 4; ++w) {
           uint32_t b0, b1;
           half4_of_e4m3x4(word(k, w), b0, b1);
-          mma_f16(c, aq[4 * i + w][0], 0u, aq[4 * i + w][1], 0u, b0, b1);
+          mma_f16(c[i], aq[4 * i + w][0], 0u, aq[4 * i + w][1], 0u, b0, b1);
         }
       }
       const float f = fq * ksc[h];
-      z[h][0] = c[0] * f;
-      z[h][1] = c[1] * f;
+      z[h][0] = (c[0][0] + c[1][0]) * f;
+      z[h][1] = (c[0][1] + c[1][1]) * f;
     }
     const int left = ctx - tile * 16 - 2 * t;               // tokens 2t + 8h + i are there while 8h + i < left
     if constexpr (edge) {                                   // tokens behind the end have no weight
