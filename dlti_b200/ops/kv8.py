@@ -10,6 +10,7 @@ the smallest for which the page's largest finite number is at most 448 scales (2
 Rows of one page are neighbours in a call, each slot occurs once (ops/_debug.py checks both)."""
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -74,12 +75,16 @@ def _check_places(op: str, pos, slots, T: int) -> None:
 
 _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 _bound: dict = {}
+_SIGNATURES = {
+    "dlti_rope_cache8": (_V, _L, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V),
+    "dlti_acc_rope_cache8": (_V, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V),
+    "dlti_paged_decode8": (_V, _L, _V, _V, _V, _V, _V, _I, _V, _I, _I, _I, _I, _I, _F, _I, _V, _V, _L, _I, _V),
+    "dlti_gather_rows8": (_V, _L, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V),
+}
 
 
-def _fn(name: str, types: tuple):
-    f = _bound.get(name)
-    if f is None:
-        f = _bound[name] = _lib.fn(name, list(types))
+def _bind(name: str):
+    f = _bound[name] = _lib.fn(name, list(_SIGNATURES[name]))
     return f
 
 
@@ -155,7 +160,7 @@ def rope_cache8_(qkv, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV,
     if out is not None:
         _check_rows("rope_cache8", dst, W)
     _check_tables(cos_t, sin_t, hd)
-    f = _fn("dlti_rope_cache8", (_V, _L, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V))
+    f = _bound.get("dlti_rope_cache8") or _bind("dlti_rope_cache8")
     _lib.check(f(qkv.data_ptr(), qkv.stride(0), dst.data_ptr(), dst.stride(0), pos.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), slots.data_ptr(),
                  k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), T, H, KV, hd, bs, _lib.dtype_code(qkv.dtype),
                  _stream(dev)), "rope_cache8")
@@ -186,7 +191,7 @@ def acc_rope_cache8(acc, dtype, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_sca
     dev = _check_device("acc_rope_cache8", acc, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale)
     _check_tables(cos_t, sin_t, hd)
     out = acc.new_empty((T, W), dtype=dtype)
-    f = _fn("dlti_acc_rope_cache8", (_V, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V))
+    f = _bound.get("dlti_acc_rope_cache8") or _bind("dlti_acc_rope_cache8")
     _lib.check(f(acc.data_ptr(), out.data_ptr(), W, pos.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), slots.data_ptr(), k8.data_ptr(), v8.data_ptr(),
                  k_scale.data_ptr(), v_scale.data_ptr(), T, H, KV, hd, bs, _lib.dtype_code(dtype), _stream(dev)), "acc_rope_cache8")
     return out
@@ -208,6 +213,7 @@ def paged_decode8_ref(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV
     return out.to(q.dtype)
 
 
+@functools.lru_cache(maxsize=4096)
 def splits8(ctas: int, reach: int) -> int:
     """CTAs over which contexts of up to `reach` tokens are cut when one each would be `ctas`: one wave of three per SM (a second one costs what it
     should save), 64 tokens at least. Up to 8 are one cluster, more are clusters of one size. us, 4 rows of 30011 tokens with 8 key heads: 6 splits
@@ -253,7 +259,7 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
     splits = splits8(B * KV * -(-(H // KV) // 8), width * bs if max_ctx is None else min(width * bs, max_ctx))
     # a workspace of this call's own: the allocator keeps it for the stream's later work, or inside the graph that captures it
     ws = torch.empty(B * H * -(-splits // 8) * (hd + 2), dtype=torch.float32, device=q.device) if splits > 8 else None
-    f = _fn("dlti_paged_decode8", (_V, _L, _V, _V, _V, _V, _V, _I, _V, _I, _I, _I, _I, _I, _F, _I, _V, _V, _L, _I, _V))
+    f = _bound.get("dlti_paged_decode8") or _bind("dlti_paged_decode8")
     _lib.check(f(q.data_ptr(), ld, k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
                  width, ctx_lens.data_ptr(), B, bs, H, KV, hd, scale, splits, None if ws is None else ws.data_ptr(),
                  out.data_ptr(), out.stride(0), _lib.dtype_code(q.dtype), _stream(dev)), "paged_decode8")
@@ -283,7 +289,7 @@ def gather_rows8_(ext, rows, slots, k8, v8, k_scale, v_scale, H, KV, hd):
         return gather_rows8_ref(ext, rows, slots, k8, v8, k_scale, v_scale, H, KV, hd)
     dev = _check_device("gather_rows8", ext, rows, slots, k8, v8, k_scale, v_scale)
     _check_rows("gather_rows8", ext, (H + 2 * KV) * hd)
-    f = _fn("dlti_gather_rows8", (_V, _L, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V))
+    f = _bound.get("dlti_gather_rows8") or _bind("dlti_gather_rows8")
     _lib.check(f(ext.data_ptr(), ext.stride(0), rows.data_ptr(), slots.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
                  v_scale.data_ptr(), slots.numel(), H, KV, hd, k8.shape[2], _lib.dtype_code(ext.dtype), _stream(dev)), "gather_rows8")
     return ext

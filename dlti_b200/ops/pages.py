@@ -8,7 +8,13 @@ import torch
 
 from . import _lib
 
-_TYPES = [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
+_call = None
+
+
+def _bind():
+    global _call
+    _call = _lib.fn("dlti_copy_pages", [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p])
+    return _call
 
 
 def check_copies(src: list[int], dst: list[int], num_pages: int) -> tuple[list[int], list[int]]:
@@ -34,6 +40,8 @@ def check_copies(src: list[int], dst: list[int], num_pages: int) -> tuple[list[i
 def _page(t: torch.Tensor, page_dim: int) -> tuple[int, int, int, int]:
     """(layers, bytes from layer to layer, bytes from page to page, bytes of a page) of a cache."""
     shape, stride, es = t.shape, t.stride(), t.element_size()
+    if t.is_contiguous() and t.numel():
+        return (shape[0], stride[0] * es, stride[1] * es, stride[1] * es) if page_dim else (1, 0, stride[0] * es, stride[0] * es)
     n = 1
     for d in range(len(shape) - 1, page_dim, -1):
         if shape[d] != 1 and stride[d] != n:
@@ -75,7 +83,7 @@ def copy_pages(caches: list[torch.Tensor], src: list[int], dst: list[int], page_
     for t in caches:
         if t.get_device() != d:
             raise ValueError(f"copy_pages: every cache is on the current device, cuda:{d}")
-    f = _lib.fn("dlti_copy_pages", _TYPES)
+    f = _call or _bind()
     what, a, b = array("q", flat), array("i", src), array("i", dst)
     _lib.check(f(what.buffer_info()[0], len(caches), a.buffer_info()[0], b.buffer_info()[0], len(a), torch._C._cuda_getCurrentRawStream(d)),
                "copy_pages")

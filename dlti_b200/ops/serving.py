@@ -293,11 +293,19 @@ def sample_given(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
     if out is None:
         out = logits.new_empty(B, dtype=torch.int64)
     lp = logits.new_empty(B, dtype=torch.float32) if want_logprob else None
-    f = _lib.fn("dlti_sample_given", _GIVEN)
-    p = [None if t is None else t.data_ptr() for t in (temperature, top_k, top_p, min_p, lp)]
-    _lib.check(f(logits.data_ptr(), ld, B, V, u.data_ptr(), p[0], p[1], p[2], p[3], out.data_ptr(), p[4], _lib.dtype_code(logits.dtype),
-                 torch._C._cuda_getCurrentRawStream(d)), "sample_given")
+    f = _given or _bind_given()
+    rc = f(logits.data_ptr(), ld, B, V, u.data_ptr(), None if temperature is None else temperature.data_ptr(),
+           None if top_k is None else top_k.data_ptr(), None if top_p is None else top_p.data_ptr(), None if min_p is None else min_p.data_ptr(),
+           out.data_ptr(), None if lp is None else lp.data_ptr(), _lib.dtype_code(logits.dtype), torch._C._cuda_getCurrentRawStream(d))
+    if rc:
+        _lib.check(rc, "sample_given")
     return out, lp
 
 
-_GIVEN = [_V, _L, _I, _I, _V, _V, _V, _V, _V, _V, _V, _I, _V]
+_given = None
+
+
+def _bind_given():
+    global _given
+    _given = _lib.fn("dlti_sample_given", [_V, _L, _I, _I, _V, _V, _V, _V, _V, _V, _V, _I, _V])
+    return _given

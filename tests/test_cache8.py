@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from dlti_b200.ops import _debug, kv8
+from dlti_b200.ops import _debug, _lib, kv8
 from dlti_b200.ops import serving as S
 from dlti_b200.ops.elementwise import rope_tables
 from . import ref_cache8 as R
@@ -459,6 +459,38 @@ def test_refusals():
     with pytest.raises(ValueError):
         kv8.gather_rows8_(x, slots[:2], slots, k8, v8, ks, vs, 4, 2, HD)
     assert rows().shape == x.shape and attend().shape == (3, 4 * HD)
+
+
+@pytest.mark.gpu
+def test_tensors_elsewhere():
+    """A tensor that is not on the current device is refused, not read."""
+    from dlti_b200.ops.pages import copy_pages
+    k8, ks = pages(4, 2, 16, 1, dev="cuda")
+    v8, vs = pages(4, 2, 16, 2, dev="cuda")
+    x = torch.zeros((3, 8 * HD), dtype=torch.bfloat16, device="cuda")
+    cos, sin = rope_tables(8, HD, 10000.0, "cuda")
+    pos, slots = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.tensor([0, 1, -1], device="cuda")
+    t, n = torch.zeros((3, 2), dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    for i in (1, 2, 3, 4, 5, 6, 7, 8):
+        a = [x, pos, cos, sin, slots, k8, v8, ks, vs]
+        a[i] = a[i].cpu()
+        with pytest.raises(ValueError):
+            kv8.rope_cache8_(*a, 4, 2, HD)
+    for i in (1, 2, 3, 4, 5, 6):
+        a = [x, k8, v8, ks, vs, t, n]
+        a[i] = a[i].cpu()
+        with pytest.raises(ValueError):
+            kv8.paged_decode8(*a, 4, 2, HD)
+    with pytest.raises(ValueError):
+        kv8.paged_decode8(x, k8, v8, ks, vs, t, n, 4, 2, HD, out=torch.zeros((3, 4 * HD), dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        kv8.gather_rows8_(x, slots[:2], slots[:2].cpu(), k8, v8, ks, vs, 4, 2, HD)
+    with pytest.raises(ValueError):
+        copy_pages([k8, v8.cpu()], [0], [1])
+    with pytest.raises(ValueError):
+        S.sample_given(x.float(), torch.zeros(3, dtype=torch.float64))
+    with pytest.raises(_lib.DltiError):
+        kv8.rope_cache8_(torch.zeros((3, 8 * HD), device="cuda"), pos, cos, sin, slots, k8, v8, ks, vs, 4, 2, HD)
 
 
 def test_index_checks():
