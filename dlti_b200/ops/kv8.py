@@ -10,7 +10,6 @@ the smallest for which the page's largest finite number is at most 448 scales (2
 Rows of one page are neighbours in a call, each slot occurs once (ops/_debug.py checks both)."""
 from __future__ import annotations
 
-import functools
 import math
 
 import torch
@@ -213,7 +212,6 @@ def paged_decode8_ref(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV
     return out.to(q.dtype)
 
 
-@functools.lru_cache(maxsize=4096)
 def splits8(ctas: int, reach: int) -> int:
     """CTAs over which contexts of up to `reach` tokens are cut when one each would be `ctas`: one wave of three per SM (a second one costs what it
     should save), 64 tokens at least. Up to 8 are one cluster, more are clusters of one size. us, 4 rows of 30011 tokens with 8 key heads: 6 splits
