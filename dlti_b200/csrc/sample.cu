@@ -16,6 +16,9 @@
 // Where the list does not hold those bins' tokens (equal logits, or logits in a narrow range) a bin is divided further by 11 bits of the logit at a
 // time, and the row read once more for each division, once for the ranks and once for the sums.
 //
+// Up to 64 long rows have a cluster of CTAs each. Every CTA reads its share of the row's chunks; largest, sums and bins are added up in each other's
+// shared memory, the list and the sums of 256 tokens go to the first CTA's, which finds the cuts and the token by itself.
+//
 // Bound by arithmetic: 256 rows of 128,000 16-bit logits with top-p 188 us, of which a row takes about 8 for the largest, 20 for sum and counts, 37 for
 // the weights, 10 for the cut (weights by the library's exp, taken again for each cut and for the draw: 396); 148 rows of greedy tokens 23.
 #include "common.cuh"
@@ -31,6 +34,7 @@ constexpr int LIST = 512, WINDOW = 7168;
 // Half of the range that is looked at first, relative to top-p's sum. The mean of a bin's bounds is off by at most 2^-9 of a token's weight, evenly
 // to either side: by 3e-5 of the sum of a thousand tokens of one weight.
 constexpr float NEAR = 3e-4f;
+constexpr int MOST_CTAS = 8;                      // of a row
 constexpr int V_MAX = 1 << 18, GROUPS = V_MAX / (32 * PER);
 constexpr double UNIT = 35184372088832.0;         // 2^45
 constexpr float RANGE = 32.f;                     // bins reach this far below the largest logit, in units of T: e^-32 < 2^-46
@@ -53,13 +57,52 @@ struct Work {
   u64 u0, u1;
   int i0, i1, g0, g1;
   uint32_t n;
+  u64 best, part[2];                              // of this CTA's share of a row, for the others of its cluster
+  double sum1;
 };
+
+// ---- a row's CTAs: a cluster that reads each its share of the chunks. The first one keeps the list and the sums and does what follows alone.
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint4 remote_u32x4(const uint32_t* p, int rank) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at_rank(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ u64 remote_u64(const void* p, int rank) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at_rank(p, rank)) : "memory");
+  return v;
+}
+// in the first CTA's memory
+template <bool SHARED>
+__device__ __forceinline__ uint32_t take_place(uint32_t* n) {
+  if constexpr (!SHARED) return atomicAdd(n, 1u);
+  uint32_t v;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(v) : "r"(at_rank(n, 0)) : "memory");
+  return v;
+}
+template <bool SHARED>
+__device__ __forceinline__ void store_first(u64* p, u64 v) {
+  if constexpr (!SHARED) *p = v;
+  else asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at_rank(p, 0)), "l"(v) : "memory");
+}
 
 template <typename T>
 struct Row {
   const T* p;
   int V;
   bool vec;
+  int rank, ctas;                                 // this CTA's share: chunks rank, rank + ctas, ...
   struct Raw {
     int4 v[sizeof(T) / 2];
   };
@@ -99,14 +142,14 @@ struct Row {
     for (int j = 0; j < PER; ++j) x[j] = fmaxf(x[j], -INFINITY);                     // NaN is -inf
   }
   __device__ __forceinline__ void get(int base, float (&x)[PER]) const { open(fetch(base), base, x); }
-  // body(chunk, base, tokens) for all of the thread's tokens; two chunks are on their way meanwhile
+  // body(chunk, base, tokens) for the thread's tokens of the CTA's share; two chunks are on their way meanwhile
   template <typename F>
   __device__ __forceinline__ void each_chunk(F&& body) const {
-    const int chunks = (V + CHUNK - 1) / CHUNK;
-    int base = threadIdx.x * PER;
-    Raw a = fetch(base), n = fetch(base + CHUNK);
-    for (int c = 0; c < chunks; ++c, base += CHUNK) {
-      const Raw m = fetch(base + 2 * CHUNK);
+    const int chunks = (V + CHUNK - 1) / CHUNK, stride = CHUNK * ctas;
+    int base = (rank * TH + threadIdx.x) * PER;
+    Raw a = fetch(base), n = fetch(base + stride);
+    for (int c = rank; c < chunks; c += ctas, base += stride) {
+      const Raw m = fetch(base + 2 * stride);
       float x[PER];
       open(a, base, x);
       body(c, base, x);
@@ -427,14 +470,14 @@ __device__ __forceinline__ int reached(Work& s, double& goal) {
   return g;
 }
 
-// Both cuts where the list is too short. by_k: the bin in which top-k ends; by_p: the bins in which top-p can, from its base to `to`.
+// Both cuts where the list is too short. by_k: the bin in which top-k ends, k_count its tokens; by_p: the bins in which top-p can, from its base to `to`.
 template <typename T>
-__device__ __noinline__ u64 cut_by_division(const Row<T> row, Work& s, const Weigh weigh, bool k_on, Group by_k, uint32_t k_left, bool p_on, Group by_p, int to,
+__device__ __noinline__ u64 cut_by_division(const Row<T> row, Work& s, const Weigh weigh, bool k_on, Group by_k, uint32_t k_count, uint32_t k_left, bool p_on, Group by_p, int to,
                                             float tp) {
   const int tid = threadIdx.x, V = row.V;
   const int chunks = (V + CHUNK - 1) / CHUNK;
   u64 floor = 0;
-  if (k_on) floor = last_kept<false>(row, s, weigh, by_k, 0ull, s.bins[by_k.g], k_left, 0.0);
+  if (k_on) floor = last_kept<false>(row, s, weigh, by_k, 0ull, k_count, k_left, 0.0);
   if (!p_on) return floor;
   for (int i = tid; i < ND; i += TH) {
     s.cnt[i] = 0;
@@ -472,7 +515,7 @@ __device__ __noinline__ u64 cut_by_division(const Row<T> row, Work& s, const Wei
 
 // The weights of a row: sums of the tokens before bin f_first, by 256 tokens (of at least `least`) and altogether, and of all; the tokens of the bins
 // from there to f_last go to the list. EVERY: top-k is off, every token's weight counts. SUM: for top-p's sum. CUT: min-p is on.
-template <bool EVERY, bool SUM, bool CUT, typename T>
+template <bool SHARED, bool EVERY, bool SUM, bool CUT, typename T>
 __device__ __noinline__ void weights(const Row<T> row, Work& s, const Weigh weigh, float f_first, float f_last, u64 least, u64& whole_, u64& sure_) {
   u64 whole = 0, sure = 0;
   row.each_chunk([&](int c, int base, const float (&x)[PER]) {
@@ -489,9 +532,9 @@ __device__ __noinline__ void weights(const Row<T> row, Work& s, const Weigh weig
     };
     auto list = [&](u64 w, float at, int j) {
       if (at >= f_first && at < f_last && base + j < row.V) {
-        const uint32_t i = atomicAdd(&s.n, 1u);
-        s.wc[i] = place(x[j], base + j);
-        s.ww[i] = w;
+        const uint32_t i = take_place<SHARED>(&s.n);
+        store_first<SHARED>(&s.wc[i], place(x[j], base + j));
+        store_first<SHARED>(&s.ww[i], w);
       }
     };
     if constexpr (EVERY) {                                             // nothing in between: eight chains of operations side by side
@@ -524,22 +567,24 @@ __device__ __noinline__ void weights(const Row<T> row, Work& s, const Weigh weig
     if (!CUT) sure += kept;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
-    if ((threadIdx.x & 31) == 0) s.cw[c * WARPS + (threadIdx.x >> 5)] = kept;
+    if ((threadIdx.x & 31) == 0) store_first<SHARED>(&s.cw[c * WARPS + (threadIdx.x >> 5)], kept);
   });
   whole_ = whole;
   sure_ = sure;
 }
 
-template <typename T>
+// SHARED: a cluster for each row
+template <typename T, bool SHARED>
 __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict__ logits, long long ld, int V, const double* __restrict__ u,
                                                              const float* __restrict__ temperature, const int* __restrict__ top_k,
                                                              const float* __restrict__ top_p, const float* __restrict__ min_p,
                                                              long long* __restrict__ out, float* __restrict__ out_logprob) {
   extern __shared__ __align__(16) unsigned char raw[];
   Work& s = *reinterpret_cast<Work*>(raw);
-  const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = SHARED ? cluster_rank() : 0, ctas = SHARED ? cluster_size() : 1;
+  const int b = blockIdx.x / ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const T* p = logits + (long long)b * ld;
-  const Row<T> row{p, V, (reinterpret_cast<uintptr_t>(p) & 15) == 0};
+  const Row<T> row{p, V, (reinterpret_cast<uintptr_t>(p) & 15) == 0, rank, ctas};
   const int chunks = (V + CHUNK - 1) / CHUNK;
 
   // the largest logit, at its lowest index
@@ -553,6 +598,7 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
         mine_at = base + j;
       }
   });
+  if (tid == 0) s.n = 0;
   u64 best = place(mine_top, mine_at);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
@@ -561,14 +607,22 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
   best = lane < WARPS ? s.red[lane] : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if constexpr (SHARED) {
+    if (tid == 0) s.best = best;
+    cluster_barrier();
+    best = remote_u64(&s.best, lane % ctas);
+#pragma unroll
+    for (int o = MOST_CTAS / 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  }
   const int arg = (int)(0xffffffffu - (uint32_t)best);
   const float top = logit_of(best);
   __syncthreads();
   if (top == -INFINITY) {                                              // nothing is left: no token is more likely than another
-    if (tid == 0) {
+    if (tid == 0 && rank == 0) {
       out[b] = 0;
       if (out_logprob) out_logprob[b] = -INFINITY;
     }
+    if constexpr (SHARED) cluster_barrier();                           // nobody leaves while others read its memory
     return;
   }
   const float t = temperature ? temperature[b] : 0.f;
@@ -585,12 +639,14 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
     for (int i = tid; i < NB; i += TH) s.bins[i] = 0;
     __syncthreads();
   }
-  float sum1 = 0.f;
+  double sum1 = 0.0;                                                   // of sums of eight in 32 bits: the same for any share, to a rounding
   if (out_logprob || k_on || p_on)
     row.each_chunk([&](int, int base, const float (&x)[PER]) {
       if (out_logprob) {
+        float some = 0.f;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) sum1 += expf(-below(top, x[j]));   // nothing for those behind the end
+        for (int j = 0; j < PER; ++j) some += expf(-below(top, x[j]));   // nothing for those behind the end
+        sum1 += (double)some;
       }
       if (k_on || p_on) {
 #pragma unroll
@@ -599,8 +655,9 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
       }
     });
   float log_sum = 0.f;
+  double whole1 = 0.0;
   if (out_logprob) {
-    double v = (double)sum1;
+    double v = sum1;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lane == 0) s.red[warp] = __double_as_longlong(v);
@@ -608,13 +665,24 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
     v = lane < WARPS ? __longlong_as_double(s.red[lane]) : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    log_sum = (float)log(v);
+    whole1 = v;
   }
+  if constexpr (SHARED) {
+    if (tid == 0) s.sum1 = whole1;
+    cluster_barrier();
+    if (out_logprob) {
+      whole1 = lane % MOST_CTAS < ctas ? __longlong_as_double((long long)remote_u64(&s.sum1, lane % MOST_CTAS)) : 0.0;
+#pragma unroll
+      for (int o = MOST_CTAS / 2; o > 0; o >>= 1) whole1 += __shfl_xor_sync(0xffffffffu, whole1, o);
+    }
+  }
+  if (out_logprob) log_sum = (float)log(whole1);
   if (!drawn) {
-    if (tid == 0) {
+    if (tid == 0 && rank == 0) {
       out[b] = arg;
       if (out_logprob) out_logprob[b] = -log_sum;
     }
+    if constexpr (SHARED) cluster_barrier();
     return;
   }
   __syncthreads();
@@ -625,11 +693,33 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
   constexpr int MINE = NB / TH;                                        // bins of a thread
   uint32_t cnt[MINE];
   if (k_on || p_on) {
+    if constexpr (SHARED) {                                            // a CTA adds up its share of the bins, then everyone reads the sums
+      const int share = NB / ctas;
+      for (int i = rank * share + 4 * tid; i < (rank + 1) * share; i += 4 * TH) {
+        uint4 c = make_uint4(0, 0, 0, 0), v[MOST_CTAS];
 #pragma unroll
-    for (int i = 0; i < MINE; ++i) cnt[i] = s.bins[MINE * tid + i];
+        for (int r = 0; r < MOST_CTAS; ++r) v[r] = r < ctas ? remote_u32x4(&s.bins[i], r) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < MOST_CTAS; ++r) c = make_uint4(c.x + v[r].x, c.y + v[r].y, c.z + v[r].z, c.w + v[r].w);
+        *reinterpret_cast<uint4*>(&s.bins[i]) = c;
+      }
+      cluster_barrier();
+      const int owner = MINE * tid / share;
+#pragma unroll
+      for (int i = 0; i < MINE; i += 4) {
+        const uint4 v = remote_u32x4(&s.bins[MINE * tid + i], owner);
+        cnt[i] = v.x;
+        cnt[i + 1] = v.y;
+        cnt[i + 2] = v.z;
+        cnt[i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) cnt[i] = s.bins[MINE * tid + i];
+    }
   }
   int k_bin = NB - 1;
-  uint32_t k_left = 0;                                                 // tokens of k_bin that top-k keeps
+  uint32_t k_left = 0, k_count = 0;                                    // tokens of k_bin that top-k keeps; its tokens
   if (k_on) {
     u64 sum = 0, all;
 #pragma unroll
@@ -639,12 +729,14 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
     for (int i = 0; i < MINE; ++i) {
       if (before < (u64)k && (u64)k <= before + cnt[i]) {
         s.i0 = MINE * tid + i;
+        s.i1 = (int)cnt[i];
         s.u0 = before;
       }
       before += cnt[i];
     }
     __syncthreads();
     k_bin = s.i0;
+    k_count = (uint32_t)s.i1;
     k_left = (uint32_t)k - (uint32_t)s.u0;
     __syncthreads();
   }
@@ -728,25 +820,40 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
     while (((near_to - near_from) >> near.shift) >= ND) ++near.shift;
   }
   bool again = n_list > WINDOW;
+  u64 whole = 0, sure = 0;                                             // weight of everything that top-p's sum counts; of the tokens before `first`
   if (!again) {
-    if (tid == 0) {
-      s.n = 0;
-      s.u0 = 0;
-    }
+    if (tid == 0) s.u0 = 0;
     __syncthreads();
-    u64 whole = 0, sure = 0;                                           // weight of everything that top-p's sum counts; of the tokens before `first`
     const float f_first = (float)first, f_last = last == NB - 1 ? INFINITY : (float)(last + 1);
     if (k_on) {
-      if (least) weights<false, false, true>(row, s, weigh, f_first, f_last, least, whole, sure);
-      else weights<false, false, false>(row, s, weigh, f_first, f_last, least, whole, sure);
+      if (least) weights<SHARED, false, false, true>(row, s, weigh, f_first, f_last, least, whole, sure);
+      else weights<SHARED, false, false, false>(row, s, weigh, f_first, f_last, least, whole, sure);
     } else if (p_on) {
-      if (least) weights<true, true, true>(row, s, weigh, f_first, f_last, least, whole, sure);
-      else weights<true, true, false>(row, s, weigh, f_first, f_last, least, whole, sure);
+      if (least) weights<SHARED, true, true, true>(row, s, weigh, f_first, f_last, least, whole, sure);
+      else weights<SHARED, true, true, false>(row, s, weigh, f_first, f_last, least, whole, sure);
     } else {
-      if (least) weights<true, false, true>(row, s, weigh, f_first, f_last, least, whole, sure);
-      else weights<true, false, false>(row, s, weigh, f_first, f_last, least, whole, sure);
+      if (least) weights<SHARED, true, false, true>(row, s, weigh, f_first, f_last, least, whole, sure);
+      else weights<SHARED, true, false, false>(row, s, weigh, f_first, f_last, least, whole, sure);
     }
     __syncthreads();
+  }
+  if constexpr (SHARED) {                                              // the first CTA goes on alone
+    whole = cta_sum(whole, s.red);
+    sure = cta_sum(sure, s.red);
+    if (tid == 0) {
+      s.part[0] = whole;
+      s.part[1] = sure;
+    }
+    cluster_barrier();
+    if (rank == 0) {
+      const bool mine = tid < ctas;
+      whole = mine ? remote_u64(&s.part[0], tid) : 0;
+      sure = mine ? remote_u64(&s.part[1], tid) : 0;
+    }
+    cluster_barrier();
+    if (rank) return;
+  }
+  if (!again) {
     n_list = s.n;
     if (first <= last && n_list <= TH) {                               // a token a thread: in order, with the weight before it
       constexpr int SORTED = WINDOW / 2;
@@ -818,7 +925,7 @@ __global__ void __launch_bounds__(TH, 1) sample_given_kernel(const T* __restrict
     __syncthreads();
   }
   if (again) {
-    const u64 floor = cut_by_division(row, s, weigh, k_on, by_k, k_left, p_on, by_p, to, tp);
+    const u64 floor = cut_by_division(row, s, weigh, k_on, by_k, k_count, k_left, p_on, by_p, to, tp);
     for (int c = 0; c < chunks; ++c) {
       const int base = c * CHUNK + tid * PER;
       float x[PER];
@@ -887,12 +994,19 @@ int launch(const void* logits, long long ld, int batch, int V, const double* u, 
   int dev = 0;
   DLTI_CUDA_CHECK(cudaGetDevice(&dev));
   if (!set[dev & 63]) {
-    DLTI_CUDA_CHECK(cudaFuncSetAttribute(sample_given_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Work)));
+    DLTI_CUDA_CHECK(cudaFuncSetAttribute(sample_given_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Work)));
+    DLTI_CUDA_CHECK(cudaFuncSetAttribute(sample_given_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Work)));
     set[dev & 63] = true;
   }
-  sample_given_kernel<T><<<batch, TH, sizeof(Work), st>>>((const T*)logits, ld, V, u, t, k, p, mp, out, lp);
+  // Several SMs for a row where there are few of them. What the CTAs tell each other takes time of its own, so a row has to be long (us for 1 / 2 / 4 / 8
+  // CTAs, of bf16 rows: one row of 32,000 31 / 33 / 29, of 99,444 in fp32 84 / 59 / 43 / 35; 32 rows of 128,000 100 / 76 / 55; 64 rows 100 / 76), and
+  // clusters of eight find room for no more than some eight rows at once (16 rows of 128,000 55 us by four, 88 by eight).
+  const int chunks = (V + CHUNK - 1) / CHUNK;
+  const int ctas = batch <= 8 && chunks >= 16 ? MOST_CTAS : batch <= 32 && chunks >= 8 ? 4 : batch <= 64 && chunks >= 16 ? 2 : 1;
+  DLTI_CUDA_CHECK(dlti_launch_pdl_cluster(DLTI_PDL_MAX_ROWS + 1, ctas, ctas > 1 ? sample_given_kernel<T, true> : sample_given_kernel<T, false>,
+                                          dim3((unsigned)(batch * ctas)), dim3(TH), sizeof(Work), st, (const T*)logits, ld, V, u, t, k, p, mp, out, lp));
   dlti_count_launch();
-  return (int)cudaGetLastError();
+  return 0;
 }
 
 }  // namespace

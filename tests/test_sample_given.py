@@ -210,6 +210,35 @@ def test_long_rows(V):
     run(torch.zeros((2, V)), uniform(2, 2), 1.0, [V - 1, 0], [1.0, 0.5], 0.0, "cuda", check_lp=False)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V", [9000, 20001, 40000, 70001])
+def test_rows_alone_and_in_batches(dev, V):
+    """A row's token is the same whatever stands beside it, however many CTAs a row of so many has: every kind of row alone and among 17, 40 and 70."""
+    x = logits(10, V, V, 1.5, torch.float32)
+    x[3] = 0.25                                                        # equal logits
+    x[4] = 1 + x[4] * 1e-4                                             # a narrow range
+    x[5, ::2], x[6] = -math.inf, -math.inf
+    x[7, V - 3] = math.inf
+    x[8, 5:V - 5] = math.nan
+    t = [1.0, 0.7, 1.3, 1.0, 1.0, 1.0, 1.0, 1.0, 2.0, 0.0]
+    k = [0, 50, V // 2, 0, V - 9, 0, 0, 0, 7, 0]
+    p = [0.95, 0.9, 0.8, 0.6, 1.0, 1.0, 0.9, 0.9, 1.0, 1.0]
+    m = [0.0, 0.0, 0.001, 0.0, 0.0, 0.01, 0.0, 0.0, 0.0, 0.0]
+    u = uniform(10, 3)
+    want = [R.token(x[b].nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf).double().tolist(), float(u[b]), t[b], k[b], p[b], m[b]) for b in range(10)]
+    to = lambda a, dt: torch.tensor(a, dtype=dt, device=dev)
+    args = (x.to(dev), u.to(dev), to(t, torch.float32), to(k, torch.int32), to(p, torch.float32), to(m, torch.float32))
+    alone = [S.sample_given(*(a[b:b + 1] for a in args), want_logprob=True) for b in range(10)]
+    assert [int(o) for o, _ in alone] == want
+    lp = torch.cat([q for _, q in alone])
+    for B in (17, 40, 70):
+        at = torch.arange(B, device=dev) % 10
+        tok, q = S.sample_given(*(a[at] for a in args), want_logprob=True)
+        assert tok.tolist() == [want[b % 10] for b in range(B)]
+        # the sums differ by the order of additions in 64 bits: by a rounding of the 32-bit logarithm (up to 12) and of a difference of it (up to 32)
+        assert torch.allclose(q, lp[at], rtol=0.0, atol=2.0 ** -20, equal_nan=True)
+
+
 def test_refusals():
     x, u = torch.zeros((3, 10)), torch.zeros(3, dtype=torch.float64)
     for kw in (dict(u=u.float()), dict(u=u[:2]), dict(temperature=torch.ones(3, dtype=torch.float64)), dict(temperature=torch.ones(2)),
