@@ -239,6 +239,32 @@ def test_rows_alone_and_in_batches(dev, V):
         assert torch.allclose(q, lp[at], rtol=0.0, atol=2.0 ** -20, equal_nan=True)
 
 
+@pytest.mark.gpu
+def test_long_rows_captured_side_by_side():
+    """Two captured calls over rows of several CTAs, replayed on two streams at once, follow what their buffers hold."""
+    xs, u = [logits(4, 70001, s).cuda() for s in range(4)], uniform(4, 6).cuda()
+    t, k, p = torch.ones(4, device="cuda"), torch.tensor([0, 300, 0, 9], dtype=torch.int32, device="cuda"), torch.full((4,), 0.9, device="cuda")
+    want = [S.sample_given(x, u, t, k, p)[0].tolist() for x in xs]
+    assert want[0] == [R.token(xs[0][b].double().tolist(), float(u[b]), 1.0, int(k[b]), float(p[b]), 0.0) for b in range(4)]
+    held = [xs[0].clone(), xs[1].clone()]
+    torch.cuda.synchronize()
+    graphs = []
+    for y in held:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            o, _ = S.sample_given(y, u, t, k, p)
+        graphs.append((gr, o))
+    held[0].copy_(xs[2])
+    held[1].copy_(xs[3])
+    torch.cuda.synchronize()
+    for s, (gr, _) in zip((torch.cuda.Stream(), torch.cuda.Stream()), graphs):
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                gr.replay()
+    torch.cuda.synchronize()
+    assert [o.tolist() for _, o in graphs] == want[2:]
+
+
 def test_refusals():
     x, u = torch.zeros((3, 10)), torch.zeros(3, dtype=torch.float64)
     for kw in (dict(u=u.float()), dict(u=u[:2]), dict(temperature=torch.ones(3, dtype=torch.float64)), dict(temperature=torch.ones(2)),
