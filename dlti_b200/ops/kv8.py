@@ -58,12 +58,14 @@ def _check_device(op: str, *tensors) -> int:
     return d
 
 
-def _check_rows(op: str, x, width: int) -> None:
+def _check_rows(op: str, x, width: int, written: bool = True) -> None:
     s = x.stride()
     if len(s) != 2 or x.shape[1] != width or s[1] != 1:
         raise ValueError(f"{op}: rows [tokens, {width}] with consecutive columns")
     if s[0] % 8 or x.data_ptr() % 16:
         raise ValueError(f"{op}: rows begin at multiples of 16 bytes")
+    if written and s[0] < width and x.shape[0] > 1:
+        raise ValueError(f"{op}: rows that are written do not overlap")
 
 
 def _check_places(op: str, pos, slots, T: int) -> None:
@@ -155,7 +157,7 @@ def rope_cache8_(qkv, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV,
     if not qkv.is_cuda:
         return rope_cache8_ref(qkv, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV, hd, out)
     dev = _check_device("rope_cache8", qkv, dst, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale)
-    _check_rows("rope_cache8", qkv, W)
+    _check_rows("rope_cache8", qkv, W, out is None)
     if out is not None:
         _check_rows("rope_cache8", dst, W)
     _check_tables(cos_t, sin_t, hd)
@@ -239,6 +241,7 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
         raise ValueError("paged_decode8: an int32 table and an int32 length for each row")
     if out is not None:
         _need(out.shape == (B, H * hd) and out.dtype == q.dtype and out.stride(1) == 1, "paged_decode8: out is [B, H hd] in q's type")
+        _need(B < 2 or out.stride(0) >= H * hd, "paged_decode8: rows that are written do not overlap")
     if _debug.ENABLED:
         _debug.check_paged("paged_decode8", block_tables, ctx_lens, k8.shape[0], k8.shape[2])
     if not q.is_cuda:

@@ -461,6 +461,35 @@ def test_refusals():
     assert rows().shape == x.shape and attend().shape == (3, 4 * HD)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rows_that_overlap(dev):
+    """Rows that are written one over the other are refused; rows that are only read may be one and the same."""
+    k8, ks = pages(4, 2, 16, 1, dev=dev)
+    v8, vs = pages(4, 2, 16, 2, dev=dev)
+    to = lambda a, dt: torch.tensor(a, dtype=dt, device=dev)
+    one = torch.ones((1, 8 * HD), dtype=torch.bfloat16, device=dev)
+    t, n = torch.zeros((3, 1), dtype=torch.int32, device=dev), to([1, 2, 3], torch.int32)
+    o = torch.zeros((1, 4 * HD), dtype=torch.bfloat16, device=dev).expand(3, -1)
+    with pytest.raises(ValueError):
+        kv8.paged_decode8(one.expand(3, -1), k8, v8, ks, vs, t, n, 4, 2, HD, out=o)
+    same = kv8.paged_decode8(one.expand(3, -1), k8, v8, ks, vs, t, n, 4, 2, HD)
+    assert torch.equal(same, kv8.paged_decode8(one.repeat(3, 1), k8, v8, ks, vs, t, n, 4, 2, HD))
+    cos, sin = rope_tables(8, HD, 10000.0, dev)
+    pos, slots = to([0, 1, 2], torch.int32), to([16, 17, 18], torch.int64)
+    out = torch.empty((3, 8 * HD), dtype=torch.bfloat16, device=dev)
+    if dev == "cuda":
+        with pytest.raises(ValueError):
+            kv8.rope_cache8_(one.expand(3, -1), pos, cos, sin, slots, k8, v8, ks, vs, 4, 2, HD)
+        with pytest.raises(ValueError):
+            kv8.rope_cache8_(out, pos, cos, sin, slots, k8, v8, ks, vs, 4, 2, HD, out=one.expand(3, -1))
+        with pytest.raises(ValueError):
+            kv8.gather_rows8_(one.expand(3, -1), slots - 16, slots, k8, v8, ks, vs, 4, 2, HD)
+    kv8.rope_cache8_(one.expand(3, -1), pos, cos, sin, slots, k8, v8, ks, vs, 4, 2, HD, out=out)
+    again = one.repeat(3, 1)
+    kv8.rope_cache8_(again, pos, cos, sin, slots, k8, v8, ks, vs, 4, 2, HD)
+    assert torch.equal(out, again)
+
+
 @pytest.mark.gpu
 def test_tensors_elsewhere():
     """A tensor that is not on the current device is refused, not read."""
