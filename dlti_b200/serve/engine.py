@@ -33,6 +33,9 @@ from .tokenizer import IncrementalDetokenizer
 _BUCKETS = [1, 2, 4, 8, 16, 32, 64, 128, 256, 512]
 
 
+GIVEN_ALL, GIVEN_SOME = 1, 2
+
+
 class StepLayout:
     """Where each per-step array lives inside ONE int64 staging buffer, so a step's metadata reaches the
     device (and the TP workers) as a single copy. T token rows = nd decode rows followed by the rows of npf
@@ -47,13 +50,14 @@ class StepLayout:
     _I32 = ("pos", "src", "ctx", "cu", "ecu", "sslot", "rseq", "segs", "topk", "temp", "topp", "minp", "tables")
 
     def __init__(self, T: int, nd: int, npf: int, mb: int, ns: int | None = None, P: int = 0, full: bool = False,
-                 nsg: int = 0, nl: int | None = None, given: bool = False):
+                 nsg: int = 0, nl: int | None = None, given: int = 0):
         """ns: prompts that are sampled in this step (default: all npf; fewer under chunked prefill, where a
         prompt's earlier chunks only fill the cache). P > 0: some prompt rows continue a prompt whose first P
         tokens (over all such prompts) are already in the paged cache: pslots[P] = their cache slots,
         pdst[P] / csrc[T - nd] = where prefix tokens / this step's prompt rows sit in the extended
         [prefix | chunk] attention layout, ecu[npf + 1] = its sequence boundaries. nl: rows whose logits are wanted
-        when that is not one per sampled sequence. given: the step brings the random numbers that its tokens are drawn with (unif) and min-p."""
+        when that is not one per sampled sequence. given: the step brings the random numbers (unif) that its tokens are drawn with, and min-p: 1 = of
+        all rows, 2 = of the rows with min-p among others (GIVEN_ALL, GIVEN_SOME)."""
         ns = npf if ns is None else ns
         self.T, self.nd, self.npf, self.mb, self.ns, self.P = T, nd, npf, mb, ns, P
         B = nd + ns
@@ -61,7 +65,7 @@ class StepLayout:
         self.n = dict(ids=T, slots=T, last=B if nl is None else nl, seeds=B, pslots=P, pdst=P, csrc=(T - nd) if P else 0,
                       pos=T, src=T, ctx=nt, cu=npf + 1 if npf else 0, ecu=npf + 1 if P else 0, sslot=nt if full else 0,
                       rseq=T if full else 0, segs=nsg, topk=B, temp=B, topp=B, tables=nt * mb)
-        self.given = given
+        self.given = int(given)
         if given:
             self.n.update(unif=B, minp=B)
         o = 0
@@ -338,9 +342,14 @@ class LLMEngine:
         ns = npf if sampled_prompts is None else sampled_prompts
         mb = max((len(t) for t in tables), default=0)
         mb = (mb + 7) & ~7
-        # min-p, or a vocabulary that `sample` does not hold: the step brings its random numbers
-        min_p = sampling[4] if sampling is not None and len(sampling) > 4 else ()
-        given = sampling is not None and (any(min_p) or (self.device.type == "cuda" and self.cfg.vocab_size > S.SAMPLE_MAX))
+        # Rows with min-p are drawn with numbers that the step brings, and all rows where `sample` does not hold the vocabulary. Both kinds may
+        # meet in a step: what a request draws is the same whatever its neighbours ask for.
+        min_p = np.asarray(sampling[4] if sampling is not None and len(sampling) > 4 else (), dtype=np.float32)   # as the rows will have it
+        given = 0
+        if sampling is not None and self.device.type == "cuda" and self.cfg.vocab_size > S.SAMPLE_MAX:
+            given = GIVEN_ALL
+        elif (min_p > 0).any():
+            given = GIVEN_ALL if (min_p > 0).all() else GIVEN_SOME
         lay = StepLayout(T, nd, npf, mb, ns, len(prefix[0]) if prefix is not None else 0, full, nsg,
                          None if want is None else len(want), given)
         slot = self._host_buffer("step", lay.words)
@@ -377,7 +386,7 @@ class LLMEngine:
         if sampling is not None:
             v["temp"][:], v["topk"][:], v["topp"][:], v["seeds"][:] = sampling[:4]
         if given:
-            v["minp"][:] = min_p if len(min_p) else 0.0
+            v["minp"][:] = min_p if min_p.size else 0.0
             v["unif"][:] = uniforms(v["seeds"])
         return PackedStep(lay, slot, int(max_seqlen), int(prefix[4]) if prefix is not None else 0, seg_at)
 
@@ -438,7 +447,7 @@ class LLMEngine:
         sampling = ([r.params.temperature for r in reqs], [r.params.top_k for r in reqs],
                     [r.params.top_p for r in reqs],
                     # random stream keyed by (request seed, index of the token being generated): same seed =>
-                    # same text, whatever else the engine is doing
+                    # same text, whatever else the engine is doing (`sample` on a GPU adds the row: the same row =>)
                     [(r.seed * 1000003 + len(r.output_ids) + r.pending) & 0x7FFFFFFFFFFFFFFF for r in reqs],
                     [r.params.min_p for r in reqs])
         return self.pack_step(nd, ids, pos, slots, ctx, tables, cu, max_seqlen, sampling, src,
@@ -481,7 +490,7 @@ class LLMEngine:
                 lay = step.layout
                 msg = np.empty(12 + lay.words, dtype=np.int64)
                 msg[:12] = [0, lay.T, lay.nd, lay.npf, lay.mb, step.max_seqlen, lay.words, int(step.want_lp), lay.ns,
-                            lay.P, step.max_ext, int(lay.given)]
+                            lay.P, step.max_ext, lay.given]
                 msg[12:] = step.slot[0][:lay.words].numpy()
                 ring.write(msg)
                 return step
@@ -489,7 +498,7 @@ class LLMEngine:
             kind, T, nd, npf, mb, max_seqlen, words, want_lp, ns, P, max_ext, given = (int(x) for x in raw[:12])
             if kind < 0:
                 return None
-            lay = StepLayout(T, nd, npf, mb, ns, P, given=bool(given))
+            lay = StepLayout(T, nd, npf, mb, ns, P, given=given)
             slot = self._host_buffer("step", words)
             slot[0][:words].numpy()[:] = raw[12:12 + words]
             step = PackedStep(lay, slot, max_seqlen, max_ext)
@@ -502,7 +511,7 @@ class LLMEngine:
                 return None
             lay = step.layout
             dist.broadcast(torch.tensor([0, lay.T, lay.nd, lay.npf, lay.mb, step.max_seqlen, lay.words,
-                                         int(step.want_lp), lay.ns, lay.P, step.max_ext, int(lay.given)], dtype=torch.int64), 0)
+                                         int(step.want_lp), lay.ns, lay.P, step.max_ext, lay.given], dtype=torch.int64), 0)
             dist.broadcast(step.slot[0][:lay.words], 0)
             return step
         hdr = torch.zeros(12, dtype=torch.int64)
@@ -510,7 +519,7 @@ class LLMEngine:
         kind, T, nd, npf, mb, max_seqlen, words, want_lp, ns, P, max_ext, given = (int(x) for x in hdr[:12])
         if kind < 0:
             return None
-        lay = StepLayout(T, nd, npf, mb, ns, P, given=bool(given))
+        lay = StepLayout(T, nd, npf, mb, ns, P, given=given)
         slot = self._host_buffer("step", words)
         dist.broadcast(slot[0][:words], 0)
         step = PackedStep(lay, slot, max_seqlen, max_ext)
@@ -547,11 +556,20 @@ class LLMEngine:
             return self._tok_dev[:0], None
         if B > self._tok_dev.numel():
             raise RuntimeError(f"{B} sampled rows exceed the sample buffer ({self._tok_dev.numel()})")
-        if step.layout.given:
-            return S.sample_given(logits, v["unif"], v["temp"], v["topk"], v["topp"], v["minp"], want_logprob=want_lp,
+        given, temp = step.layout.given, v["temp"]
+        if given == GIVEN_ALL:
+            return S.sample_given(logits, v["unif"], temp, v["topk"], v["topp"], v["minp"], want_logprob=want_lp,
                                   out=self._tok_dev[:B])
-        toks, lps = S.sample(logits, v["temp"], v["topk"], v["topp"], v["seeds"], step=0, want_logprob=want_lp,
+        other = None
+        if given:                                          # each of the two takes the other's rows as greedy ones, which cost least
+            other = v["minp"] > 0
+            own, own_lps = S.sample_given(logits, v["unif"], temp.masked_fill(~other, 0.0), v["topk"], v["topp"], v["minp"], want_logprob=want_lp)
+            temp = temp.masked_fill(other, 0.0)
+        toks, lps = S.sample(logits, temp, v["topk"], v["topp"], v["seeds"], step=0, want_logprob=want_lp,
                              out=self._tok_dev[:B])
+        if given:
+            torch.where(other, own, toks, out=toks)
+            lps = torch.where(other, own_lps, lps) if want_lp else None
         return toks, lps
 
     def _decode_graph(self, step: "PackedStep"):
@@ -563,7 +581,7 @@ class LLMEngine:
         dev, mbs = self.device, self.max_blocks_per_seq
         g = self.graphs.get(bucket)
         if g is None:
-            glay = StepLayout(bucket, bucket, 0, mbs, full=self.per_sequence, given=True)
+            glay = StepLayout(bucket, bucket, 0, mbs, full=self.per_sequence, given=GIVEN_ALL)
             buf = torch.zeros(glay.words, dtype=torch.int64, device=dev)
             st = glay.views(buf, torch)
             st["slots"].fill_(-1)

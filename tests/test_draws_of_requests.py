@@ -1,0 +1,113 @@
+"""What a request draws is its own matter: its seed, its settings and its place among the answers to a prompt, not what runs beside it."""
+import json
+import os
+import socket
+import subprocess
+import sys
+
+import pytest
+
+from dlti_b200.serve.params import SamplingParams
+from .test_cache8_serving import DEVICES, engine, prompts
+
+
+def run(eng, requests, late=4):
+    """requests: (id, prompt, params, whether it joins after `late` steps). The tokens and log-probabilities of each."""
+    for rid, p, sp, _ in (r for r in requests if not r[3]):
+        eng.add_request(list(p), sp, rid)
+    for _ in range(late):
+        eng.step()
+    for rid, p, sp, _ in (r for r in requests if r[3]):
+        eng.add_request(list(p), sp, rid)
+    while eng.has_unfinished():
+        eng.step()
+    return {r[0]: (list(eng.requests[r[0]].output_ids), list(eng.requests[r[0]].logprobs)) for r in requests}
+
+
+@pytest.mark.parametrize("graphs", [False, pytest.param(True, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("mine", [0.0, 0.03])
+def test_a_seeded_request_beside_neighbours(dev, graphs, mine, monkeypatch):
+    """A request with or without min-p, beside a neighbour that joins late, ends early, and has min-p or not: the same tokens and log-probabilities."""
+    import dlti_b200.ops.gemm as G
+    monkeypatch.setattr(G, "_SKINNY_SPLIT", 1)               # a summation order that does not change from run to run
+    if graphs and dev == "cpu":
+        pytest.skip("graphs are captured on a GPU")
+    p, q = prompts([12, 30], 2)
+    got = []
+    for theirs in (0.0, 1e-50, 0.05, 1.0):                   # (1e-50 is none in the 32 bits that a row has for it)
+        a = SamplingParams(max_tokens=20, temperature=1.5, top_p=0.95, min_p=mine, seed=5, ignore_eos=True, logprobs=1)
+        b = SamplingParams(max_tokens=7, temperature=0.0, min_p=theirs, ignore_eos=True)
+        got.append(run(engine(dev, graphs=graphs), [("a", p, a, False), ("b", q, b, True)]))
+    assert len(got[0]["a"][0]) == 20 and len(set(got[0]["a"][0])) > 3
+    for g in got[1:]:
+        assert g["a"] == got[0]["a"] and g["b"][0] == got[0]["b"][0]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rows_of_both_kinds_in_one_step(dev, monkeypatch):
+    """Requests with min-p between others without, drawn and greedy: each has the tokens that it has where all are of one kind in its step."""
+    import dlti_b200.ops.gemm as G
+    monkeypatch.setattr(G, "_SKINNY_SPLIT", 1)
+    ps = prompts([12, 30, 5, 21], 3)
+    sps = [SamplingParams(max_tokens=8, temperature=t, min_p=m, top_k=40, seed=9 + i, ignore_eos=True)
+           for i, (t, m) in enumerate(((1.2, 0.0), (1.4, 0.02), (0.0, 0.0), (0.0, 0.3)))]
+
+    def take(change):
+        out = engine(dev, async_scheduling=False).generate(ps, [SamplingParams(**{**vars(s), **change(s)}) for s in sps])
+        return [o["token_ids"] for o in out]
+
+    mixed = take(lambda s: {})
+    off = take(lambda s: {"min_p": 0.0})                     # as many rows of the same prompts, all by `sample`
+    on = take(lambda s: {"min_p": s.min_p or 0.02})          # and all by `sample_given`
+    assert [mixed[0], mixed[1], mixed[2], mixed[3]] == [off[0], on[1], off[2], on[3]] and mixed[0] != on[0] and mixed[1] != off[1]
+
+
+TWO = r"""
+import json, sys, torch
+sys.path.insert(0, {root!r})
+from dlti_b200.models.config import PRESETS
+from dlti_b200.parallel import comm
+from dlti_b200.serve.engine import LLMEngine
+from dlti_b200.serve.model_runner import TPContext, TPWeights
+from dlti_b200.serve.params import SamplingParams
+from dlti_b200.serve.tokenizer import ByteTokenizer
+info = comm.init_distributed("cpu")
+cfg = PRESETS["tiny"]
+w = TPWeights(cfg, info.rank, info.world_size, "cpu", torch.float32).init_random(5)
+for l in w.layers:
+    for k in ("w_qkv", "w_o", "w_gu", "w_down"):
+        l[k].mul_(4.0)
+w.embed.mul_(4.0); w.lm_head.mul_(4.0)
+eng = LLMEngine(cfg, w, TPContext(info, "nccl", None, cfg), ByteTokenizer(cfg.vocab_size), info=info, num_blocks=20, max_model_len=256, use_cuda_graphs=False)
+if info.rank != 0:
+    eng.worker_loop()
+else:
+    sps = [SamplingParams(max_tokens=n, temperature=1.3, min_p=m, seed=3, ignore_eos=True, logprobs=1) for n, m in ((12, 0.0), (6, 0.04), (9, 0.0))]
+    out = eng.generate([[1] + list(range(40, 40 + n)) for n in (5, 33, 20)], sps)
+    eng.shutdown_workers()
+    json.dump([o["token_ids"] for o in out], open(sys.argv[1], "w"))
+comm.shutdown()
+"""
+
+
+@pytest.mark.parametrize("control", ["shm", "gloo"])
+def test_steps_of_both_kinds_on_two_ranks(tmp_path, control):
+    """Every rank draws a step's rows the same way (gloo, two processes): the tokens of one process."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    script = tmp_path / "two.py"
+    script.write_text(TWO.format(root=root))
+    env = dict(os.environ, PYTHONPATH=root, OMP_NUM_THREADS="2", DLTI_TP_CONTROL=control)
+    out = []
+    for world in (1, 2):
+        to = tmp_path / f"{world}.json"
+        cmd, e = [sys.executable, str(script), str(to)], dict(env, WORLD_SIZE="1", RANK="0", LOCAL_RANK="0")
+        if world == 2:
+            with socket.socket() as so:
+                so.bind(("127.0.0.1", 0))
+                port = so.getsockname()[1]
+            cmd, e = [sys.executable, "-m", "dlti_b200.launch", "--num_gpus=2", f"--master_port={port}", "--no_local_rank", str(script), str(to)], env
+        r = subprocess.run(cmd, env=e, capture_output=True, text=True, timeout=300, cwd=root)
+        assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+        out.append(json.load(open(to)))
+    assert out[0] == out[1] and [len(t) for t in out[0]] == [12, 6, 9]
