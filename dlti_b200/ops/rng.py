@@ -35,12 +35,13 @@ def philox4x32(c0, c1, c2, c3, k0, k1):
     return c0, c1, c2, c3
 
 
-def uniforms(seeds) -> np.ndarray:
-    """A number in [0, 1) of 53 bits for each 64-bit seed (float64): the first two words of Philox keyed by the seed."""
+def uniforms(seeds, answers=0) -> np.ndarray:
+    """A number in [0, 1) of 53 bits for each 64-bit seed (float64): the first two words of Philox keyed by the seed. answers: a number for each (or
+    one for all) that counts, so that one seed gives several numbers."""
     s = np.asarray(seeds, dtype=np.int64).astype(np.uint64)
     z = np.zeros_like(s)
     with np.errstate(over="ignore"):
-        a, b, _, _ = philox4x32(z, z, z, z + np.uint64(0x5A18), s & _MASK, s >> _S32)
+        a, b, _, _ = philox4x32(z + np.asarray(answers, dtype=np.uint64), z, z, z + np.uint64(0x5A18), s & _MASK, s >> _S32)
     return ((a >> np.uint64(5)).astype(np.float64) * 67108864.0 + (b >> np.uint64(6)).astype(np.float64)) / 9007199254740992.0
 
 

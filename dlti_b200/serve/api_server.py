@@ -318,9 +318,10 @@ def _params_from_body(b: dict) -> SamplingParams:
 
 
 def _answer(sp: SamplingParams, base_id: str, idx: int) -> SamplingParams:
-    """Parameters of answer idx of a request: n answers to each prompt follow one another, and all but the first may go on from its pages."""
+    """Parameters of answer idx of a request: n answers to each prompt follow one another, and all but the first may go on from its pages.
+    With a seed, each draws numbers of its own."""
     first = idx // sp.n * sp.n
-    return SamplingParams(**{**vars(sp), "fork_of": None if idx == first else f"{base_id}-{first}"})
+    return SamplingParams(**{**vars(sp), "answer": idx - first, "fork_of": None if idx == first else f"{base_id}-{first}"})
 
 
 def _error(message: str, typ: str = "invalid_request_error", code: int = 400):

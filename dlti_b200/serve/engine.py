@@ -323,7 +323,7 @@ class LLMEngine:
                   want=None) -> "PackedStep":
         """Lay one step's metadata out in a pinned host buffer (see StepLayout). ids/pos/slots cover all T
         rows (decode rows first); ctx/tables the nd decode rows; cu the packed prompts (relative to row nd);
-        sampling = (temperature, top_k, top_p, seeds[, min_p]) per sampled row or None. sampled_prompts: how many of the
+        sampling = (temperature, top_k, top_p, seeds[, min_p, answers]) per sampled row or None. sampled_prompts: how many of the
         prompts (the first ones) end in this step; prefix = (pslots, pdst, csrc, ecu, max_ext) when prompt rows
         continue prompts whose earlier tokens are in the cache.
         For a runner with per_sequence = True, ctx / tables / sslots (state slots) cover the prompts too and starts[i]
@@ -387,7 +387,7 @@ class LLMEngine:
             v["temp"][:], v["topk"][:], v["topp"][:], v["seeds"][:] = sampling[:4]
         if given:
             v["minp"][:] = min_p if min_p.size else 0.0
-            v["unif"][:] = uniforms(v["seeds"])
+            v["unif"][:] = uniforms(v["seeds"], sampling[5] if len(sampling) > 5 else 0)
         return PackedStep(lay, slot, int(max_seqlen), int(prefix[4]) if prefix is not None else 0, seg_at)
 
     def _pack_batch(self, batch: Batch, want=None, given: dict | None = None) -> "PackedStep":
@@ -449,7 +449,7 @@ class LLMEngine:
                     # random stream keyed by (request seed, index of the token being generated): same seed =>
                     # same text, whatever else the engine is doing (`sample` on a GPU adds the row: the same row =>)
                     [(r.seed * 1000003 + len(r.output_ids) + r.pending) & 0x7FFFFFFFFFFFFFFF for r in reqs],
-                    [r.params.min_p for r in reqs])
+                    [r.params.min_p for r in reqs], [r.params.answer for r in reqs])
         return self.pack_step(nd, ids, pos, slots, ctx, tables, cu, max_seqlen, sampling, src,
                               sampled_prompts=batch.num_sampled - nd, prefix=prefix, sslots=sslots, starts=starts,
                               want=want)

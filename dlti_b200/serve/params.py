@@ -23,6 +23,7 @@ class SamplingParams:
     echo: bool = False
     skip_special_tokens: bool = True
     detokenize: bool = True     # False (vLLM's field of the same name): return token ids only, produce no text
+    answer: int = 0             # place among the n answers to one prompt: with one seed each draws numbers of its own (min-p, long vocabularies)
     fork_of: str | None = None  # request with the same prompt whose pages this one may share (LLMEngine(fork_samples=True))
 
     def __post_init__(self):
@@ -34,7 +35,7 @@ class SamplingParams:
         if self.max_tokens is None:
             self.max_tokens = 16
         if (self.temperature < 0 or not (0 < self.top_p <= 1.0) or not (0 <= self.min_p <= 1.0) or self.max_tokens < 1
-                or self.n < 1):
+                or self.n < 1 or self.answer < 0):
             raise ValueError("invalid sampling parameters")
 
 

@@ -111,3 +111,64 @@ def test_steps_of_both_kinds_on_two_ranks(tmp_path, control):
         assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
         out.append(json.load(open(to)))
     assert out[0] == out[1] and [len(t) for t in out[0]] == [12, 6, 9]
+
+
+def test_answers_to_one_seeded_prompt():
+    """Through the API: with a seed, the n answers of a request with min-p differ from one another, repeat from call to call, and the first one is
+    the answer to n = 1. Streams and chats, too."""
+    pytest.importorskip("fastapi")
+    from fastapi.testclient import TestClient
+
+    from dlti_b200.serve.api_server import AsyncEngine, build_app
+    eng = engine(fork_samples=True)
+    aeng = AsyncEngine(eng)
+    aeng.start()
+    try:
+        with TestClient(build_app(aeng, "tiny")) as c:
+            def texts(**more):
+                ask = {"prompt": prompts([20, 9], 1), "max_tokens": 8, "n": 3, "temperature": 1.5, "min_p": 0.02, "ignore_eos": True, "seed": 4, **more}
+                chat = more.pop("chat", None)
+                if chat:
+                    ask = {"messages": [{"role": "user", "content": "hello"}], **{k: v for k, v in ask.items() if k not in ("prompt", "chat")}}
+                r = c.post("/v1/chat/completions" if chat else "/v1/completions", json=ask)
+                out = {}
+                if more.get("stream"):
+                    parts = [json.loads(x[6:]) for x in r.text.split("\n\n") if x.startswith("data: {")]
+                else:
+                    parts = [r.json()]
+                for ch in (ch for part in parts for ch in part["choices"]):
+                    out[ch["index"]] = out.get(ch["index"], "") + (ch.get("text") or (ch.get("message") or ch.get("delta") or {}).get("content") or "")
+                return [out[i] for i in sorted(out)]
+
+            first = texts()
+            assert len(set(first)) == 6 and texts() == first and texts(stream=True) == first
+            assert texts(n=1) == first[::3] and texts(seed=5) != first
+            talk = texts(chat=True)
+            assert len(set(talk)) == 3 and texts(chat=True, stream=True) == talk and texts(chat=True, n=1) == talk[:1]
+    finally:
+        aeng.stop = True
+        aeng.thread.join(timeout=10)
+    assert eng.sched.num_forks > 0
+
+
+@pytest.mark.parametrize("dev,vocab,min_p", [("cpu", None, 0.02), pytest.param("cuda", None, 0.02, marks=pytest.mark.gpu),
+                                             pytest.param("cuda", 60032, 0.0, marks=pytest.mark.gpu)])
+def test_places_among_the_answers(dev, vocab, min_p):
+    """One seed, four places: four texts, also where a long vocabulary is what brings the numbers; a place is none of its row's."""
+    p = prompts([14], 4)[0]
+    sp = [SamplingParams(max_tokens=10, temperature=1.5, min_p=min_p, seed=2 ** 62 + 7, answer=i, ignore_eos=True) for i in range(4)]
+    got = engine(dev, vocab=vocab, max_num_seqs=8).generate([p] * 4, sp)
+    assert len({tuple(o["token_ids"]) for o in got}) == 4
+    with pytest.raises(ValueError):
+        SamplingParams(answer=-1)
+    if dev == "cpu":
+        back = engine(dev).generate([p] * 4, sp[::-1])
+        assert [o["token_ids"] for o in back[::-1]] == [o["token_ids"] for o in got]
+
+
+def test_numbers_of_a_seed():
+    from dlti_b200.ops.rng import uniforms
+    s = list(range(500)) + [2 ** 63 - 1]
+    a = [uniforms(s, i).tolist() for i in range(5)]
+    assert a[0] == uniforms(s).tolist() and len({x for r in a for x in r}) == 5 * 501
+    assert uniforms([3, 3, 9], [0, 4, 1]).tolist() == [a[0][3], a[4][3], a[1][9]]
