@@ -827,6 +827,16 @@ bool sizes_ok(const char* what, int H, int KV, int hd, int bs) {
   dlti_set_error(msg);
   return false;
 }
+// What the kernels read and write in pieces of `unit` bytes: addresses, and the pitch of rows in elements of two bytes.
+bool begins_ok(const char* what, std::initializer_list<const void*> at, long long pitch, int unit = 16) {
+  bool ok = pitch % 8 == 0;
+  for (const void* p : at) ok &= reinterpret_cast<uintptr_t>(p) % unit == 0;
+  if (ok) return true;
+  char msg[160];
+  std::snprintf(msg, sizeof msg, "%s: rows, pages, rotation tables and accumulators begin at multiples of %d bytes", what, unit);
+  dlti_set_error(msg);
+  return false;
+}
 
 }  // namespace
 
@@ -838,6 +848,7 @@ DLTI_API int dlti_rope_cache8(const void* x, long long x_ld, void* out, long lon
   if (!sizes_ok("rope_cache8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
   if (tokens <= 0) return 0;
   if (tokens > 1 << 24) return DLTI_ERR_TOO_LARGE;
+  if (!begins_ok("rope_cache8", {x, out, cos_t, sin_t, k8, v8}, x_ld | out_ld)) return DLTI_ERR_BAD_ARG;
   const Rows8 p{x, out, x_ld, out_ld, pos, cos_t, sin_t, slots, (uint8_t*)k8, (uint8_t*)v8, ks, vs, (int)tokens, H, KV, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs)};
   if (dtype == DLTI_BF16) return rows8_t<__nv_bfloat16, false>(p, st);
   if (dtype == DLTI_FP16) return rows8_t<__half, false>(p, st);
@@ -851,6 +862,7 @@ DLTI_API int dlti_acc_rope_cache8(float* acc, void* out, long long out_ld, const
   if (!sizes_ok("acc_rope_cache8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
   if (tokens <= 0) return 0;
   if (tokens > 1 << 24) return DLTI_ERR_TOO_LARGE;
+  if (!begins_ok("acc_rope_cache8", {acc, out, cos_t, sin_t, k8, v8}, out_ld)) return DLTI_ERR_BAD_ARG;
   const Rows8 p{acc, out, (long long)(H + 2 * KV) * HD, out_ld, pos, cos_t, sin_t, slots, (uint8_t*)k8, (uint8_t*)v8, ks, vs, (int)tokens, H, KV, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs)};
   if (dtype == DLTI_BF16) return rows8_t<__nv_bfloat16, true>(p, st);
   if (dtype == DLTI_FP16) return rows8_t<__half, true>(p, st);
@@ -869,6 +881,7 @@ DLTI_API int dlti_paged_decode8(const void* q, long long q_ld, const void* k8, c
   if (batch <= 0) return 0;
   const int parts = (splits + 7) / 8;
   if (batch > 65535 || splits < 1 || parts > MAX_PARTS || splits % parts || (parts > 1 && !workspace)) return DLTI_ERR_BAD_ARG;
+  if (!begins_ok("paged_decode8", {q, k8, v8}, q_ld)) return DLTI_ERR_BAD_ARG;
   const Attend8 p{q, q_ld, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, tables, ctx, max_blocks, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs),
                   H / KV, KV, splits, parts, scale * 1.4426950408889634f, workspace, workspace + (long long)batch * H * parts * HD, out, out_ld};
   if (dtype == DLTI_BF16) return attend8_t<__nv_bfloat16>(p, batch, st);
@@ -882,6 +895,7 @@ DLTI_API int dlti_gather_rows8(void* ext, long long ext_ld, const long long* row
   if (!sizes_ok("gather_rows8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
   if (n <= 0) return 0;
   if (n > 1 << 30) return DLTI_ERR_TOO_LARGE;
+  if (!begins_ok("gather_rows8", {ext}, ext_ld) || !begins_ok("gather_rows8", {k8, v8}, 0, 8)) return DLTI_ERR_BAD_ARG;
   const dim3 grid((unsigned)((n + 7) / 8), (unsigned)((2 * KV + 15) / 16));
   if (dtype == DLTI_BF16)
     gather8_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((__nv_bfloat16*)ext, ext_ld, rows, slots, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, (int)n, H, KV, bs);
