@@ -191,6 +191,7 @@ def sample_ref(logits, temperature, top_k, top_p, generator=None):
 
 
 SAMPLE_MAX = 51200           # longest row of `sample` on a GPU (it is held in shared memory)
+SAMPLE_GIVEN_MAX = 1 << 18   # of `sample_given`
 
 
 def sample(logits, temperature=None, top_k=None, top_p=None, seeds=None, step: int = 0, want_logprob=False,
@@ -278,8 +279,8 @@ def sample_given(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
             raise ValueError(f"sample_given: {name} is {dt} [{B}]")
     if out is not None and (out.dtype is not torch.int64 or out.shape != (B,) or not out.is_contiguous()):
         raise ValueError(f"sample_given: out is int64 [{B}]")
-    if not 1 <= V <= 1 << 18:
-        raise ValueError(f"sample_given: rows of 1 to 262144 logits, got {V}")
+    if not 1 <= V <= SAMPLE_GIVEN_MAX:
+        raise ValueError(f"sample_given: rows of 1 to {SAMPLE_GIVEN_MAX} logits, got {V}")
     if not logits.is_cuda:
         tok, lp = sample_given_ref(logits, u, temperature, top_k, top_p, min_p)
         return tok if out is None else out.copy_(tok), lp if want_logprob else None

@@ -265,6 +265,8 @@ class LLMEngine:
     def add_request(self, prompt: str | list[int], params: SamplingParams | None = None,
                     request_id: str | None = None) -> str:
         params = params or SamplingParams()
+        if self.cfg.vocab_size > S.SAMPLE_GIVEN_MAX and (params.min_p > 0 or self.device.type == "cuda"):   # given tokens (replay) are not drawn
+            raise ValueError(f"tokens are drawn from at most {S.SAMPLE_GIVEN_MAX} logits, not {self.cfg.vocab_size}")
         ids = list(prompt) if not isinstance(prompt, str) else self.tokenizer.encode(prompt)
         if not ids:
             ids = [self.cfg.bos_token_id]

@@ -172,3 +172,26 @@ def test_numbers_of_a_seed():
     a = [uniforms(s, i).tolist() for i in range(5)]
     assert a[0] == uniforms(s).tolist() and len({x for r in a for x in r}) == 5 * 501
     assert uniforms([3, 3, 9], [0, 4, 1]).tolist() == [a[0][3], a[4][3], a[1][9]]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_vocabularies_that_no_sampler_holds(dev):
+    """More logits than a row can be drawn from: a request is refused when it comes, not in the engine's next step, and nothing of it stays. On the
+    host that is so for requests with min-p. Replays, which draw nothing, go on."""
+    from dlti_b200.serve.params import Request
+    eng = engine(dev, vocab=262144 + 64)
+    p = prompts([5], 1)[0]
+    for m in (0.1, 0.0) if dev == "cuda" else (0.1,):
+        with pytest.raises(ValueError, match="262144"):
+            eng.add_request(p, SamplingParams(min_p=m), "r")
+    assert not eng.has_unfinished() and not eng.requests
+    if dev == "cpu":
+        assert len(eng.generate([p], SamplingParams(max_tokens=2, temperature=1.0, seed=1, ignore_eos=True))[0]["token_ids"]) == 2
+    assert eng.replay_step([(Request("s", [], SamplingParams()), p, [4])]).shape == (1, 262144 + 64)
+
+
+@pytest.mark.gpu
+def test_the_longest_vocabulary():
+    eng = engine("cuda", vocab=262144, graphs=True)
+    out = eng.generate(prompts([5, 9], 1), [SamplingParams(max_tokens=4, temperature=t, min_p=0.001, seed=1, ignore_eos=True) for t in (0.0, 1.0)])
+    assert all(len(o["token_ids"]) == 4 and max(o["token_ids"]) < 262144 for o in out)
