@@ -103,10 +103,18 @@ class Scheduler:
             return False
         return self._origin(r) is not None or any(p.request_id == r.params.fork_of and p.prompt_ids == r.prompt_ids for p in admitted)
 
+    @staticmethod
+    def _ready(origin: Request | None) -> bool:
+        """Whether forks can start from it: its whole prompt is in the cache, or on its way in a step that is launched."""
+        return origin is not None and origin.prefill_done and origin.sched_tokens > len(origin.prompt_ids)
+
     def _admit_forks(self, decode: list[Request], room: int) -> list[tuple[int, int]]:
         """Waiting requests whose origin has its whole prompt in the cache join the decode rows (at most `room`): they share the pages of all prompt
         tokens but the last, which is their first row. Ones whose origin is still at its prompt wait for it; the others stay as they were. Returns
-        the pages to copy."""
+        the pages to copy.
+
+        Forks pass requests that came before them, as their origin's pages are there only while it runs: a prompt that waits for pages is kept back by
+        the forks of what was running before it, no others. One that finds no room is passed by nobody that came after it."""
         copies = []
         if not self.fork_samples:
             return copies
@@ -114,7 +122,7 @@ class Scheduler:
             if room <= 0 or len(self.running) >= self.max_num_seqs:
                 break
             p = self._origin(r)
-            if p is None or not p.prefill_done or p.sched_tokens <= len(p.prompt_ids):
+            if not self._ready(p):
                 continue
             n = len(r.prompt_ids)
             if not self.blocks.can_allocate(n + 1, (n - 1) // self.blocks.block_size):
@@ -173,6 +181,8 @@ class Scheduler:
             if r.pending:                         # preempted with a sampled token still unread: next step
                 break
             if self._waits_for_origin(r, admitted):
+                if self._ready(self._origin(r)):  # it found no room: what comes free is its own
+                    break
                 held.append(self.waiting.popleft())
                 continue
             n = r.num_tokens                      # prompt (+ already generated tokens if it was preempted)
@@ -245,6 +255,8 @@ class Scheduler:
             if r.pending:
                 break
             if self._waits_for_origin(r, admitted):
+                if self._ready(self._origin(r)):  # it found no room: what comes free is its own
+                    break
                 held.append(self.waiting.popleft())
                 continue
             r.num_computed, r.prefill_done = self._take_cached_prefix(r), False
