@@ -176,7 +176,8 @@ class LLMEngine:
                  fork_samples: bool = False):
         """kv_cache_dtype: "auto" keeps keys and values in the compute type, "fp8" in 8 bits with a scale for each page and head (Llama family):
         half the memory and half the bytes a decode step reads. fork_samples: a request whose params.fork_of names a running one with the same
-        prompt shares that prompt's pages instead of running it again (the n answers of one API request)."""
+        prompt shares that prompt's pages instead of running it again (the n answers of one API request); its first row reads them from the cache,
+        with "fp8" in 8 bits."""
         self.cfg, self.w, self.tp, self.tokenizer, self.info = cfg, weights, tp, tokenizer, info
         self.device = weights.embed.device
         self.dtype = weights.embed.dtype
