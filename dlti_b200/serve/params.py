@@ -12,7 +12,6 @@ class SamplingParams:
     temperature: float = 1.0
     top_p: float = 1.0
     top_k: int = 0              # 0 / -1 = off
-    min_p: float = 0.0          # tokens less likely than min_p times the likeliest are not drawn (0 = off)
     n: int = 1
     seed: int | None = None
     stop: list[str] = field(default_factory=list)
@@ -23,6 +22,7 @@ class SamplingParams:
     echo: bool = False
     skip_special_tokens: bool = True
     detokenize: bool = True     # False (vLLM's field of the same name): return token ids only, produce no text
+    min_p: float = 0.0          # tokens less likely than min_p times the likeliest are not drawn (0 = off)
     answer: int = 0             # place among the n answers to one prompt: with one seed each draws numbers of its own (min-p, long vocabularies)
     fork_of: str | None = None  # request with the same prompt whose pages this one may share (LLMEngine(fork_samples=True))
 

@@ -195,3 +195,13 @@ def test_the_longest_vocabulary():
     eng = engine("cuda", vocab=262144, graphs=True)
     out = eng.generate(prompts([5, 9], 1), [SamplingParams(max_tokens=4, temperature=t, min_p=0.001, seed=1, ignore_eos=True) for t in (0.0, 1.0)])
     assert all(len(o["token_ids"]) == 4 and max(o["token_ids"]) < 262144 for o in out)
+
+
+def test_sampling_parameters_by_place():
+    """Their order, for calls that give them by place: what came later comes last."""
+    import dataclasses
+    names = [f.name for f in dataclasses.fields(SamplingParams)]
+    assert names[:14] == ["max_tokens", "temperature", "top_p", "top_k", "n", "seed", "stop", "stop_token_ids", "ignore_eos", "min_tokens", "logprobs", "echo",
+                          "skip_special_tokens", "detokenize"]
+    sp = SamplingParams(8, 0.7, 0.9, 40, 1, 42, ["x"])
+    assert (sp.n, sp.seed, sp.stop, sp.min_p) == (1, 42, ["x"], 0.0)
