@@ -181,6 +181,7 @@ class LLMEngine:
         self.cfg, self.w, self.tp, self.tokenizer, self.info = cfg, weights, tp, tokenizer, info
         self.device = weights.embed.device
         self.dtype = weights.embed.dtype
+        self.long_rows = self.device.type == "cuda" and cfg.vocab_size > S.SAMPLE_MAX      # logits that `sample` does not hold
         self.max_model_len = max_model_len or cfg.max_position_embeddings
         self.rank = tp.rank
         self.world = tp.world
@@ -326,7 +327,7 @@ class LLMEngine:
                   want=None) -> "PackedStep":
         """Lay one step's metadata out in a pinned host buffer (see StepLayout). ids/pos/slots cover all T
         rows (decode rows first); ctx/tables the nd decode rows; cu the packed prompts (relative to row nd);
-        sampling = (temperature, top_k, top_p, seeds[, min_p, answers]) per sampled row or None. sampled_prompts: how many of the
+        sampling = (temperature, top_k, top_p, seeds[, min_p, places among the answers]) per sampled row or None. sampled_prompts: how many of the
         prompts (the first ones) end in this step; prefix = (pslots, pdst, csrc, ecu, max_ext) when prompt rows
         continue prompts whose earlier tokens are in the cache.
         For a runner with per_sequence = True, ctx / tables / sslots (state slots) cover the prompts too and starts[i]
@@ -347,12 +348,13 @@ class LLMEngine:
         mb = (mb + 7) & ~7
         # Rows with min-p are drawn with numbers that the step brings, and all rows where `sample` does not hold the vocabulary. Both kinds may
         # meet in a step: what a request draws is the same whatever its neighbours ask for.
-        min_p = np.asarray(sampling[4] if sampling is not None and len(sampling) > 4 else (), dtype=np.float32)   # as the rows will have it
+        min_p, answers = (*sampling[4:], *(0.0, 0)[len(sampling) - 4:]) if sampling is not None else (0.0, 0)
         given = 0
-        if sampling is not None and self.device.type == "cuda" and self.cfg.vocab_size > S.SAMPLE_MAX:
+        if sampling is not None and self.long_rows:
             given = GIVEN_ALL
-        elif (min_p > 0).any():
-            given = GIVEN_ALL if (min_p > 0).all() else GIVEN_SOME
+        elif min_p:
+            some = np.asarray(min_p, dtype=np.float32) > 0         # as the rows will have it
+            given = GIVEN_ALL if some.all() else GIVEN_SOME if some.any() else 0
         lay = StepLayout(T, nd, npf, mb, ns, len(prefix[0]) if prefix is not None else 0, full, nsg,
                          None if want is None else len(want), given)
         slot = self._host_buffer("step", lay.words)
@@ -389,8 +391,8 @@ class LLMEngine:
         if sampling is not None:
             v["temp"][:], v["topk"][:], v["topp"][:], v["seeds"][:] = sampling[:4]
         if given:
-            v["minp"][:] = min_p if min_p.size else 0.0
-            v["unif"][:] = uniforms(v["seeds"], sampling[5] if len(sampling) > 5 else 0)
+            v["minp"][:] = min_p
+            v["unif"][:] = uniforms(v["seeds"], answers)
         return PackedStep(lay, slot, int(max_seqlen), int(prefix[4]) if prefix is not None else 0, seg_at)
 
     def _pack_batch(self, batch: Batch, want=None, given: dict | None = None) -> "PackedStep":
@@ -451,8 +453,10 @@ class LLMEngine:
                     [r.params.top_p for r in reqs],
                     # random stream keyed by (request seed, index of the token being generated): same seed =>
                     # same text, whatever else the engine is doing (`sample` on a GPU adds the row: the same row =>)
-                    [(r.seed * 1000003 + len(r.output_ids) + r.pending) & 0x7FFFFFFFFFFFFFFF for r in reqs],
-                    [r.params.min_p for r in reqs], [r.params.answer for r in reqs])
+                    [(r.seed * 1000003 + len(r.output_ids) + r.pending) & 0x7FFFFFFFFFFFFFFF for r in reqs])
+        min_p = [r.params.min_p for r in reqs]
+        if self.long_rows or any(min_p):
+            sampling += (min_p, [r.params.answer for r in reqs])
         return self.pack_step(nd, ids, pos, slots, ctx, tables, cu, max_seqlen, sampling, src,
                               sampled_prompts=batch.num_sampled - nd, prefix=prefix, sslots=sslots, starts=starts,
                               want=want)

@@ -205,3 +205,17 @@ def test_sampling_parameters_by_place():
                           "skip_special_tokens", "detokenize"]
     sp = SamplingParams(8, 0.7, 0.9, 40, 1, 42, ["x"])
     assert (sp.n, sp.seed, sp.stop, sp.min_p) == (1, 42, ["x"], 0.0)
+
+
+def test_settings_of_a_packed_step():
+    """With and without min-p and places, as pack_step takes them."""
+    from dlti_b200.ops.rng import uniforms
+    eng = engine()
+    row = ([0.7, 0.0], [0, 3], [1.0, 0.5], [11, 12])
+    pack = lambda *more: eng.pack_step(2, [4, 5], [0, 0], [0, 16], [1, 1], [[0], [1]], [], 0, (*row, *more))
+    assert [pack(*m).layout.given for m in ((), ([0.0, 0.0],), ([0.1, 0.0],), ([0.1, 0.2],), ([0.1, 1e-50], [0, 2]))] == [0, 0, 2, 1, 2]
+    import numpy as np
+    for more, want in ((([0.1, 0.0],), uniforms([11, 12])), (([0.1, 0.0], [3, 1]), uniforms([11, 12], [3, 1]))):
+        step = pack(*more)
+        v = step.layout.views(step.slot[0].numpy(), np)
+        assert v["unif"].tolist() == want.tolist() and v["minp"].tolist() == [np.float32(0.1), 0.0] and v["seeds"].tolist() == row[3]
