@@ -837,6 +837,21 @@ bool begins_ok(const char* what, std::initializer_list<const void*> at, long lon
   dlti_set_error(msg);
   return false;
 }
+// Rows that are written (b) are the rows they are made from (a), or share no memory with them: blocks of rows have no order among them. Pitches and
+// widths in bytes.
+bool apart_ok(const char* what, const void* a_, long long la, long long wa, const void* b_, long long lb, long long wb, long long rows) {
+  const long long a = (long long)reinterpret_cast<uintptr_t>(a_), b = (long long)reinterpret_cast<uintptr_t>(b_);
+  if (rows == 1) la = lb = 0;
+  if ((a == b && la == lb) || b >= a + (rows - 1) * la + wa || a >= b + (rows - 1) * lb + wb) return true;
+  if (la == lb && la > 0) {                       // columns side by side
+    const long long d = ((b - a) % la + la) % la;
+    if (d >= wa && d <= la - wb) return true;
+  }
+  char msg[120];
+  std::snprintf(msg, sizeof msg, "%s: rows that are written overlap other rows that are read", what);
+  dlti_set_error(msg);
+  return false;
+}
 
 }  // namespace
 
@@ -848,7 +863,10 @@ DLTI_API int dlti_rope_cache8(const void* x, long long x_ld, void* out, long lon
   if (!sizes_ok("rope_cache8", H, KV, hd, bs)) return DLTI_ERR_UNSUPPORTED;
   if (tokens <= 0) return 0;
   if (tokens > 1 << 24) return DLTI_ERR_TOO_LARGE;
-  if (!begins_ok("rope_cache8", {x, out, cos_t, sin_t, k8, v8}, x_ld | out_ld)) return DLTI_ERR_BAD_ARG;
+  const long long width = 2LL * (H + 2 * KV) * HD;
+  if (!begins_ok("rope_cache8", {x, out, cos_t, sin_t, k8, v8}, x_ld | out_ld) ||
+      !apart_ok("rope_cache8", x, 2 * x_ld, width, out, 2 * out_ld, width, tokens))
+    return DLTI_ERR_BAD_ARG;
   const Rows8 p{x, out, x_ld, out_ld, pos, cos_t, sin_t, slots, (uint8_t*)k8, (uint8_t*)v8, ks, vs, (int)tokens, H, KV, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs)};
   if (dtype == DLTI_BF16) return rows8_t<__nv_bfloat16, false>(p, st);
   if (dtype == DLTI_FP16) return rows8_t<__half, false>(p, st);
@@ -881,7 +899,8 @@ DLTI_API int dlti_paged_decode8(const void* q, long long q_ld, const void* k8, c
   if (batch <= 0) return 0;
   const int parts = (splits + 7) / 8;
   if (batch > 65535 || splits < 1 || parts > MAX_PARTS || splits % parts || (parts > 1 && !workspace)) return DLTI_ERR_BAD_ARG;
-  if (!begins_ok("paged_decode8", {q, k8, v8}, q_ld)) return DLTI_ERR_BAD_ARG;
+  if (!begins_ok("paged_decode8", {q, k8, v8}, q_ld) || !apart_ok("paged_decode8", q, 2 * q_ld, 2LL * H * HD, out, 2 * out_ld, 2LL * H * HD, batch))
+    return DLTI_ERR_BAD_ARG;
   const Attend8 p{q, q_ld, (const uint8_t*)k8, (const uint8_t*)v8, ks, vs, tables, ctx, max_blocks, bs, (bs & (bs - 1)) ? -1 : __builtin_ctz(bs),
                   H / KV, KV, splits, parts, scale * 1.4426950408889634f, workspace, workspace + (long long)batch * H * parts * HD, out, out_ld};
   if (dtype == DLTI_BF16) return attend8_t<__nv_bfloat16>(p, batch, st);

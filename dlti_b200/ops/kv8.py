@@ -150,8 +150,8 @@ def rope_cache8_ref(qkv, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, 
 
 
 def rope_cache8_(qkv, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV, hd, out=None):
-    """Rotate q and k of every token row of qkv [T, (H + 2 KV) hd] in place, or from qkv into `out`, which then gets v too; write rotated k and v
-    of the rows with a slot (int64 [T], -1 = none) to the 8-bit pages. Returns the rotated rows."""
+    """Rotate q and k of every token row of qkv [T, (H + 2 KV) hd] in place, or from qkv into `out` (qkv itself or apart from it), which then gets v
+    too; write rotated k and v of the rows with a slot (int64 [T], -1 = none) to the 8-bit pages. Returns the rotated rows."""
     dst = qkv if out is None else out
     bs = k8.shape[2]
     _check_cache("rope_cache8", k8, v8, k_scale, v_scale, H, KV, hd)
@@ -242,7 +242,8 @@ def splits8(ctas: int, reach: int) -> int:
 
 def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd, scale=None, out=None, max_ctx: int | None = None):
     """paged_decode over 8-bit pages. q: [B, >= H hd] (row b = the single new token of sequence b); block_tables int32 [B, *], ctx_lens int32 [B],
-    0 = a row of zeros; max_ctx: the longest context that may occur (a context beyond it is read in full). Returns out [B, H hd]."""
+    0 = a row of zeros; max_ctx: the longest context that may occur (a context beyond it is read in full). Returns out [B, H hd]: a tensor of its own,
+    or the one given, which is the queries' own place or apart from them."""
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     _check_cache("paged_decode8", k8, v8, k_scale, v_scale, H, KV, hd)
     B, W = q.shape

@@ -357,7 +357,8 @@ int dlti_sample(const void* logits, long long ld, int batch, int V, const float*
 int dlti_sample_given(const void* logits, long long ld, int batch, int V, const double* u, const float* temperature, const int* top_k,
                       const float* top_p, const float* min_p, long long* out, float* out_logprob, int dtype, dlti_stream_t stream);
 /* Cache in 8 bits (csrc/kv8.cu): pages [num_blocks, KV, block_size, 128] e4m3 with scales [num_blocks, KV], powers of two. Rows of one page are
- * consecutive, a slot occurs once (-1: none). A row at place 0 begins its page; any other may raise its scale. out may be x. Rows, pages, rotation
+ * consecutive, a slot occurs once (-1: none). A row at place 0 begins its page; any other may raise its scale. out may be x, or the queries; it
+ * is apart from them otherwise (refused if not). Rows, pages, rotation
  * tables and accumulators begin at multiples of 16 bytes, pitches are multiples of 8 elements: refused otherwise. */
 int dlti_rope_cache8(const void* x, long long x_ld, void* out, long long out_ld, const int* pos, const float* cos_t, const float* sin_t,
                      const long long* slots, void* k8, void* v8, float* ks, float* vs, long long tokens, int H, int KV, int hd, int bs, int dtype,
