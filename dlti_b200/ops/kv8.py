@@ -69,11 +69,10 @@ def _check_rows(op: str, x, width: int, written: bool = True) -> None:
         raise ValueError(f"{op}: rows that are written do not overlap")
 
 
-def _check_begin(op: str, what: str, *tensors, unit: int = 16) -> None:
+def _check_begin(op: str, k8, v8, unit: int = 16) -> None:
     """The kernels read and write pieces of `unit` bytes."""
-    for t in tensors:
-        if t.data_ptr() % unit:
-            raise ValueError(f"{op}: {what} begin at multiples of {unit} bytes")
+    if (k8.data_ptr() | v8.data_ptr()) % unit:
+        raise ValueError(f"{op}: pages begin at multiples of {unit} bytes")
 
 
 def _check_places(op: str, pos, slots, T: int) -> None:
@@ -168,7 +167,7 @@ def rope_cache8_(qkv, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV,
     _check_rows("rope_cache8", qkv, W, out is None)
     if out is not None:
         _check_rows("rope_cache8", dst, W)
-    _check_begin("rope_cache8", "pages", k8, v8)
+    _check_begin("rope_cache8", k8, v8)
     _check_tables(cos_t, sin_t, hd)
     f = _bound.get("dlti_rope_cache8") or _bind("dlti_rope_cache8")
     _lib.check(f(qkv.data_ptr(), qkv.stride(0), dst.data_ptr(), dst.stride(0), pos.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), slots.data_ptr(),
@@ -181,7 +180,7 @@ def _check_tables(cos_t, sin_t, hd: int) -> None:
     if not (cos_t.shape == sin_t.shape and cos_t.shape[1] == hd // 2 and cos_t.dtype is sin_t.dtype is torch.float32 and cos_t.is_contiguous()
             and sin_t.is_contiguous()):
         raise ValueError(f"rotation tables are float32 [positions, {hd // 2}]")
-    if cos_t.data_ptr() % 16 or sin_t.data_ptr() % 16:
+    if (cos_t.data_ptr() | sin_t.data_ptr()) % 16:
         raise ValueError("rotation tables begin at multiples of 16 bytes")
 
 
@@ -201,7 +200,8 @@ def acc_rope_cache8(acc, dtype, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_sca
         acc.zero_()
         return out
     dev = _check_device("acc_rope_cache8", acc, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale)
-    _check_begin("acc_rope_cache8", "accumulator and pages", acc, k8, v8)
+    _check_begin("acc_rope_cache8", k8, v8)
+    _need(acc.data_ptr() % 16 == 0, "acc_rope_cache8: the accumulator begins at a multiple of 16 bytes")
     _check_tables(cos_t, sin_t, hd)
     out = acc.new_empty((T, W), dtype=dtype)
     f = _bound.get("dlti_acc_rope_cache8") or _bind("dlti_acc_rope_cache8")
@@ -264,7 +264,7 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
     ld, unit = q.stride()
     if unit != 1 or ld % 8 or q.data_ptr() % 16:
         raise ValueError("paged_decode8: rows begin at multiples of 16 bytes")
-    _check_begin("paged_decode8", "pages", k8, v8)
+    _check_begin("paged_decode8", k8, v8)
     bs, width = k8.shape[2], block_tables.shape[1]
     _need(width * bs < 1 << 31, "paged_decode8: contexts have 31 bits")
     if out is None:
@@ -304,7 +304,7 @@ def gather_rows8_(ext, rows, slots, k8, v8, k_scale, v_scale, H, KV, hd):
         return gather_rows8_ref(ext, rows, slots, k8, v8, k_scale, v_scale, H, KV, hd)
     dev = _check_device("gather_rows8", ext, rows, slots, k8, v8, k_scale, v_scale)
     _check_rows("gather_rows8", ext, (H + 2 * KV) * hd)
-    _check_begin("gather_rows8", "pages", k8, v8, unit=8)
+    _check_begin("gather_rows8", k8, v8, unit=8)
     f = _bound.get("dlti_gather_rows8") or _bind("dlti_gather_rows8")
     _lib.check(f(ext.data_ptr(), ext.stride(0), rows.data_ptr(), slots.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
                  v_scale.data_ptr(), slots.numel(), H, KV, hd, k8.shape[2], _lib.dtype_code(ext.dtype), _stream(dev)), "gather_rows8")
