@@ -62,8 +62,9 @@ __device__ __forceinline__ int4 pack8(const float (&f)[8]) {
 // has two rows at a time. A CTA takes a block of rows, whose angles it keeps in shared memory in the rows' type, and a share of the heads. Of
 // keys and values a warp takes all rows of one page (consecutive rows with slots in it) for one head, so nobody else touches that head's piece of
 // the page or its scale; a page that goes on behind the block is done by the CTA in whose block it begins. Up to 16 rows are in flight and stay in
-// registers between finding the scale and rounding to it. Bound by a warp's loads and arithmetic taking turns: 6,506 rows of 48 heads 40 us (182 MB,
-// 4.5 TB/s; the first form, a warp of rows at a time with angles from global memory, 64); a CTA more an SM, or one less, 47 and 50.
+// registers between finding the scale and rounding to it. Bound by a warp's loads and arithmetic taking turns: 6,506 rows of 48 heads 40 us, a call
+// among others (182 MB, 4.5 TB/s; in place the same; the first form, a warp of rows at a time with angles from global memory, 64); a CTA more an SM, or
+// one less, 47 and 50.
 // ---------------------------------------------------------------------------------------------
 struct Rows8 {
   const void* x;                 // [tokens, x_ld] in the rows' type, or the fp32 accumulator [tokens, (H + 2 KV) * 128], left zero
@@ -333,12 +334,19 @@ __global__ void __launch_bounds__(256, C::CTAS) rows8_kernel(const Rows8 p) {
 template <typename T, bool ACC>
 int rows8_t(const Rows8& p, cudaStream_t st) {
   const int heads = p.H + 2 * p.KV, eights = (heads + 7) / 8;
+  // A row a block up to the size of most decode steps, whose rows have a page each: sixteen of them would take turns. us of a call alone (cold L2, 6 of
+  // them the launch's, read to 2), a row a block / sixteen rows, 32 query and 8 key heads: decode rows 1 8/10, 8 10/27, 64 10/45, 256 14/45, 512 20/47;
+  // rows of one prompt 8 12/10, 16 16/12, 128 16/12, 256 20/14, 512 23/14. Their number does not tell them apart: a prompt of up to 256 rows alone
+  // takes 4 to 6 us more than it could, a step of more than 256 decode rows 27.
   if (p.tokens <= DLTI_PDL_MAX_ROWS) {
     DLTI_CUDA_CHECK(dlti_launch_pdl(p.tokens, rows8_kernel<T, ACC, DecodeRows>, dim3((unsigned)p.tokens, (unsigned)eights), dim3(256), 0, st, p));
   } else {
     const int blocks = (p.tokens + PromptRows::ROWS - 1) / PromptRows::ROWS;
     const long long ctas = (long long)blocks * eights;
-    const int share = ctas <= 3 * 148 ? 1 : ctas <= 10 * 148 ? 2 : 4;      // heads of a warp
+    // Heads of a warp: few blocks need every SM, many serve their angles to more heads. us as above for 1 / 2 / 4 heads, 32 query and 32 key heads: 495
+    // rows (372 CTAs) 20/29/41, 993 (756) 25/29/37, 1,989 (1,500) 39/41/42, 3,979 64/65/63, 7,959 117/111/106; 64 and 8 heads: 495 (310) 20/24/25, 993
+    // (630) 25/22/25, 1,989 (1,250) 33/30/29, 3,979 (2,490) 51/47/45, 7,959 90/78/76.
+    const int share = ctas <= 3 * 148 ? 1 : ctas <= 10 * 148 ? 2 : 4;
     DLTI_CUDA_CHECK(dlti_launch_pdl(p.tokens, rows8_kernel<T, ACC, PromptRows>, dim3((unsigned)blocks, (unsigned)((eights + share - 1) / share)), dim3(256),
                                     0, st, p));
   }
@@ -359,8 +367,9 @@ int rows8_t(const Rows8& p, cudaStream_t st) {
 //   queries: scaled by a power of two per head so that their 16 bits are fp16 numbers exactly (down to 2^-39 of the head's largest);
 //   weights p s_v: p <= 1 times the page's value scale over the largest seen so far, as fp16 hi + lo, rows g and g + 8 of the same product:
 //   22 bits, absolutely 2^-40 of the largest.
-// Bound by HBM: 128 rows of up to 2,048 tokens with 32 key heads 299 us (1.62 GB, 5.4 TB/s; through registers instead of the ring 503), 4 rows of
-// 30,011 with 8 key heads 49 us. Three CTAs an SM at 168 registers: four spill (370 instead of 257).
+// Bound by HBM: 128 rows of up to 2,048 tokens with 32 key heads 293 us in a loop over fresh inputs (1.62 GB, 5.5 TB/s; through registers instead of the
+// ring 503), 4 rows of up to 30,011 with 8 key heads 49 us. Three CTAs an SM at 168 registers: four spill (the first case over one set of inputs, which
+// stays warm in part: 370 instead of 257).
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"

@@ -3,7 +3,7 @@
 // A token has to be the one that exact arithmetic gives, also where a cut or the drawn number falls close to a border: with n kept tokens a
 // relative error of d in the running sums moves about one draw in 1 / (2 n d), which for sums in 32 bits is one in a hundred over a whole
 // vocabulary. So weights exp((x - max) / T) are taken in double precision and held as whole numbers of 2^-45: their sums are exact, do not depend
-// on the order of atomics, and with up to 2^18 of them stay below 2^63.
+// on the order of atomics, and with up to 2^18 of them are at most 2^63, in 64 bits without a sign.
 //
 // The kept tokens are a prefix of the order (logit descending, index ascending); each cut is found as the last token that it keeps, a 64-bit
 // number of the logit's order-preserving bits and the index. A CTA takes a row and reads it three times, after the first time from L2:
@@ -19,8 +19,10 @@
 // Up to 64 long rows have a cluster of CTAs each. Every CTA reads its share of the row's chunks; largest, sums and bins are added up in each other's
 // shared memory, the list and the sums of 256 tokens go to the first CTA's, which finds the cuts and the token by itself.
 //
-// Bound by arithmetic: 256 rows of 128,000 16-bit logits with top-p 188 us, of which a row takes about 8 for the largest, 20 for sum and counts, 37 for
-// the weights, 10 for the cut (weights by the library's exp, taken again for each cut and for the draw: 396); 148 rows of greedy tokens 23.
+// Bound by arithmetic: 256 rows of 128,000 16-bit logits with top-p 188 us a call among others (weights by the library's exp, taken again for each cut
+// and for the draw: 396). One row an SM, 148 of them, a call alone with a cold L2: 104 us, of which 6 are the launch's, 18 go to the largest logit (25 us
+// is what greedy tokens take), 12 to the log-probability's sum, 16 to counts and bounds, 41 to the weights, 10 to the cut and the draw (by leaving out
+// what follows each); the second 108 rows take as long again, 197 in all.
 #include "common.cuh"
 
 namespace {

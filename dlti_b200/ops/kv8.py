@@ -87,12 +87,13 @@ _SIGNATURES = {
     "dlti_rope_cache8": (_V, _L, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V),
     "dlti_acc_rope_cache8": (_V, _V, _L, _V, _V, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V),
     "dlti_paged_decode8": (_V, _L, _V, _V, _V, _V, _V, _I, _V, _I, _I, _I, _I, _I, _F, _I, _V, _V, _L, _I, _V),
+    "dlti_paged_decode8_floats": (_I, _I, _I),
     "dlti_gather_rows8": (_V, _L, _V, _V, _V, _V, _V, _V, _L, _I, _I, _I, _I, _I, _V),
 }
 
 
 def _bind(name: str):
-    f = _bound[name] = _lib.fn(name, list(_SIGNATURES[name]))
+    f = _bound[name] = _lib.fn(name, list(_SIGNATURES[name]), _L if name.endswith("_floats") else _I)
     return f
 
 
@@ -228,11 +229,15 @@ def paged_decode8_ref(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV
 
 def splits8(ctas: int, reach: int) -> int:
     """CTAs over which contexts of up to `reach` tokens are cut when one each would be `ctas`: one wave of three per SM (a second one costs what it
-    should save), 64 tokens at least. Up to 8 are one cluster, more are clusters of one size. us, 4 rows of 30011 tokens with 8 key heads: 6 splits
-    72, 8 59, 12 57, 16 (two waves) 70; 32 rows of 4000 tokens with 4 key heads: 1 split 49, 2 41, 3 37, 4 (two waves) 49."""
+    should save), 64 tokens at least. Up to 8 are one cluster, more are clusters of one size.
+
+    us of a call alone, from a graph and with a cold L2, 6 of them the launch's, read to 2: 4 rows of up to 30011 tokens with 8 key heads in 6 splits
+    72, 8 61, 12 59, 16 (two waves) 72; 32 rows of 4000 tokens with 4 key heads in 1 split 49, 2 39, 3 37, 4 (two waves) 47; 64 rows of up to 1000
+    with 4 key heads in 1 split 22, 2 (two waves) 31."""
     n = max(1, min(128, 3 * 148 // max(1, ctas), -(-reach // 64)))
-    # 9 .. 15 of short contexts: one cluster and no kernel to join two (700 tokens with 32 key heads: 19 us in 10 splits, 15 in 8; but 4 rows of
-    # 30011 tokens with 8 key heads: 47 us in 12, 61 in 8)
+    # 9 .. 15 splits of short contexts: 8, one cluster and no kernel to join two. Measured as above, in 8 / in 12: 4 rows with 8 key heads of 700 tokens
+    # 14 / 16, 2000 16 / 18, 4000 20 / 22, 8000 27 / 29, 12000 33 / 35, 16000 41 / 41, 30011 61 / 59; one row with 32 key heads of 4000 18 / 20,
+    # 6000 22 / 25, 8000 27 / 27, 16000 41 / 39. So the border could lie up to 16000; between, it costs 2 us at most.
     if n < 16 and reach <= 4096:
         return min(n, 8)
     while n % -(-n // 8):
@@ -273,7 +278,7 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
         _check_device("paged_decode8", out)
     splits = splits8(B * KV * -(-(H // KV) // 8), width * bs if max_ctx is None else min(width * bs, max_ctx))
     # a workspace of this call's own: the allocator keeps it for the stream's later work, or inside the graph that captures it
-    ws = torch.empty(B * H * -(-splits // 8) * (hd + 2), dtype=torch.float32, device=q.device) if splits > 8 else None
+    ws = torch.empty((_bound.get("dlti_paged_decode8_floats") or _bind("dlti_paged_decode8_floats"))(B, H, splits), dtype=torch.float32, device=q.device) if splits > 8 else None
     f = _bound.get("dlti_paged_decode8") or _bind("dlti_paged_decode8")
     _lib.check(f(q.data_ptr(), ld, k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
                  width, ctx_lens.data_ptr(), B, bs, H, KV, hd, scale, splits, None if ws is None else ws.data_ptr(),
