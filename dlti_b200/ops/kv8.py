@@ -69,10 +69,12 @@ def _check_rows(op: str, x, width: int, written: bool = True) -> None:
         raise ValueError(f"{op}: rows that are written do not overlap")
 
 
-def _check_begin(op: str, k8, v8, unit: int = 16) -> None:
-    """The kernels read and write pieces of `unit` bytes."""
-    if (k8.data_ptr() | v8.data_ptr()) % unit:
+def _pages(op: str, k8, v8, unit: int = 16) -> tuple[int, int]:
+    """Addresses of the pages, which the kernels read and write in pieces of `unit` bytes."""
+    k, v = k8.data_ptr(), v8.data_ptr()
+    if (k | v) % unit:
         raise ValueError(f"{op}: pages begin at multiples of {unit} bytes")
+    return k, v
 
 
 def _check_places(op: str, pos, slots, T: int) -> None:
@@ -168,21 +170,23 @@ def rope_cache8_(qkv, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV,
     _check_rows("rope_cache8", qkv, W, out is None)
     if out is not None:
         _check_rows("rope_cache8", dst, W)
-    _check_begin("rope_cache8", k8, v8)
-    _check_tables(cos_t, sin_t, hd)
+    kp, vp = _pages("rope_cache8", k8, v8)
+    cp, sp = _tables(cos_t, sin_t, hd)
     f = _bound.get("dlti_rope_cache8") or _bind("dlti_rope_cache8")
-    _lib.check(f(qkv.data_ptr(), qkv.stride(0), dst.data_ptr(), dst.stride(0), pos.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), slots.data_ptr(),
-                 k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), T, H, KV, hd, bs, _lib.dtype_code(qkv.dtype),
+    _lib.check(f(qkv.data_ptr(), qkv.stride(0), dst.data_ptr(), dst.stride(0), pos.data_ptr(), cp, sp, slots.data_ptr(),
+                 kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), T, H, KV, hd, bs, _lib.dtype_code(qkv.dtype),
                  _stream(dev)), "rope_cache8")
     return dst
 
 
-def _check_tables(cos_t, sin_t, hd: int) -> None:
+def _tables(cos_t, sin_t, hd: int) -> tuple[int, int]:
     if not (cos_t.shape == sin_t.shape and cos_t.shape[1] == hd // 2 and cos_t.dtype is sin_t.dtype is torch.float32 and cos_t.is_contiguous()
             and sin_t.is_contiguous()):
         raise ValueError(f"rotation tables are float32 [positions, {hd // 2}]")
-    if (cos_t.data_ptr() | sin_t.data_ptr()) % 16:
+    c, s = cos_t.data_ptr(), sin_t.data_ptr()
+    if (c | s) % 16:
         raise ValueError("rotation tables begin at multiples of 16 bytes")
+    return c, s
 
 
 def acc_rope_cache8(acc, dtype, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale, H, KV, hd):
@@ -201,12 +205,12 @@ def acc_rope_cache8(acc, dtype, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_sca
         acc.zero_()
         return out
     dev = _check_device("acc_rope_cache8", acc, pos, cos_t, sin_t, slots, k8, v8, k_scale, v_scale)
-    _check_begin("acc_rope_cache8", k8, v8)
+    kp, vp = _pages("acc_rope_cache8", k8, v8)
     _need(acc.data_ptr() % 16 == 0, "acc_rope_cache8: the accumulator begins at a multiple of 16 bytes")
-    _check_tables(cos_t, sin_t, hd)
+    cp, sp = _tables(cos_t, sin_t, hd)
     out = acc.new_empty((T, W), dtype=dtype)
     f = _bound.get("dlti_acc_rope_cache8") or _bind("dlti_acc_rope_cache8")
-    _lib.check(f(acc.data_ptr(), out.data_ptr(), W, pos.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), slots.data_ptr(), k8.data_ptr(), v8.data_ptr(),
+    _lib.check(f(acc.data_ptr(), out.data_ptr(), W, pos.data_ptr(), cp, sp, slots.data_ptr(), kp, vp,
                  k_scale.data_ptr(), v_scale.data_ptr(), T, H, KV, hd, bs, _lib.dtype_code(dtype), _stream(dev)), "acc_rope_cache8")
     return out
 
@@ -269,7 +273,7 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
     ld, unit = q.stride()
     if unit != 1 or ld % 8 or q.data_ptr() % 16:
         raise ValueError("paged_decode8: rows begin at multiples of 16 bytes")
-    _check_begin("paged_decode8", k8, v8)
+    kp, vp = _pages("paged_decode8", k8, v8)
     bs, width = k8.shape[2], block_tables.shape[1]
     _need(width * bs < 1 << 31, "paged_decode8: contexts have 31 bits")
     if out is None:
@@ -280,7 +284,7 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
     # a workspace of this call's own: the allocator keeps it for the stream's later work, or inside the graph that captures it
     ws = torch.empty((_bound.get("dlti_paged_decode8_floats") or _bind("dlti_paged_decode8_floats"))(B, H, splits), dtype=torch.float32, device=q.device) if splits > 8 else None
     f = _bound.get("dlti_paged_decode8") or _bind("dlti_paged_decode8")
-    _lib.check(f(q.data_ptr(), ld, k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+    _lib.check(f(q.data_ptr(), ld, kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
                  width, ctx_lens.data_ptr(), B, bs, H, KV, hd, scale, splits, None if ws is None else ws.data_ptr(),
                  out.data_ptr(), out.stride(0), _lib.dtype_code(q.dtype), _stream(dev)), "paged_decode8")
     return out
@@ -309,8 +313,8 @@ def gather_rows8_(ext, rows, slots, k8, v8, k_scale, v_scale, H, KV, hd):
         return gather_rows8_ref(ext, rows, slots, k8, v8, k_scale, v_scale, H, KV, hd)
     dev = _check_device("gather_rows8", ext, rows, slots, k8, v8, k_scale, v_scale)
     _check_rows("gather_rows8", ext, (H + 2 * KV) * hd)
-    _check_begin("gather_rows8", k8, v8, unit=8)
+    kp, vp = _pages("gather_rows8", k8, v8, unit=8)
     f = _bound.get("dlti_gather_rows8") or _bind("dlti_gather_rows8")
-    _lib.check(f(ext.data_ptr(), ext.stride(0), rows.data_ptr(), slots.data_ptr(), k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(),
+    _lib.check(f(ext.data_ptr(), ext.stride(0), rows.data_ptr(), slots.data_ptr(), kp, vp, k_scale.data_ptr(),
                  v_scale.data_ptr(), slots.numel(), H, KV, hd, k8.shape[2], _lib.dtype_code(ext.dtype), _stream(dev)), "gather_rows8")
     return ext
