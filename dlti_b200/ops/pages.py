@@ -37,10 +37,12 @@ def check_copies(src: list[int], dst: list[int], num_pages: int) -> tuple[list[i
     return src, dst
 
 
-def _page(t: torch.Tensor, page_dim: int) -> tuple[int, int, int, int]:
-    """(layers, bytes from layer to layer, bytes from page to page, bytes of a page) of a cache."""
+def _page(t: torch.Tensor, page_dim: int) -> tuple[int, ...]:
+    """(layers, bytes from layer to layer, bytes from page to page, bytes of a page) of a cache; () if nothing is in it."""
     shape, stride, es = t.shape, t.stride(), t.element_size()
-    if t.is_contiguous() and t.numel():
+    if t.is_contiguous():                                    # as all that hold nothing are
+        if not t.numel():
+            return ()
         return (shape[0], stride[0] * es, stride[1] * es, stride[1] * es) if page_dim else (1, 0, stride[0] * es, stride[0] * es)
     n = 1
     for d in range(len(shape) - 1, page_dim, -1):
@@ -67,9 +69,11 @@ def copy_pages(caches: list[torch.Tensor], src: list[int], dst: list[int], page_
     src, dst = check_copies(src, dst, num)
     flat = []
     for t in caches:
-        flat.append(t.data_ptr())
-        flat += _page(t, page_dim)
-    if not src:
+        page = _page(t, page_dim)
+        if page:
+            flat.append(t.data_ptr())
+            flat += page
+    if not src or not flat:
         return
     if not caches[0].is_cuda:
         a, b = torch.tensor(src), torch.tensor(dst)
@@ -85,5 +89,5 @@ def copy_pages(caches: list[torch.Tensor], src: list[int], dst: list[int], page_
             raise ValueError(f"copy_pages: every cache is on the current device, cuda:{d}")
     f = _call or _bind()
     what, a, b = array("q", flat), array("i", src), array("i", dst)
-    _lib.check(f(what.buffer_info()[0], len(caches), a.buffer_info()[0], b.buffer_info()[0], len(a), torch._C._cuda_getCurrentRawStream(d)),
+    _lib.check(f(what.buffer_info()[0], len(flat) // 5, a.buffer_info()[0], b.buffer_info()[0], len(a), torch._C._cuda_getCurrentRawStream(d)),
                "copy_pages")

@@ -64,3 +64,18 @@ def test_refusals():
         with pytest.raises(ValueError):
             copy_pages(caches, [0], [1], page_dim=dim)
     assert check_copies([1, 2, 2], [1, 3, 4], 5) == ([2, 2], [3, 4])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_caches_of_nothing(dev):
+    """Caches without layers, pages without numbers and caches without pages beside others: nothing of them is copied, the others are."""
+    a = filled((3, 5, 40), 1, dev)
+    want = a.clone()
+    want[:, 4], want[:, 0] = a[:, 1], a[:, 2]
+    empty = [torch.zeros(s, device=dev) for s in ((0, 5, 8), (3, 5, 0), (3, 5, 4, 0, 2))]
+    copy_pages([empty[0], a, *empty[1:]], [1, 2], [4, 0], page_dim=1)
+    assert torch.equal(a, want)
+    copy_pages(empty, [1, 2], [4, 0], page_dim=1)
+    copy_pages([torch.zeros((0, 4), device=dev)], [], [])
+    with pytest.raises(ValueError):
+        copy_pages([torch.zeros((3, 0, 4), device=dev)], [0], [1], page_dim=1)
