@@ -282,7 +282,10 @@ def paged_decode8(q, k8, v8, k_scale, v_scale, block_tables, ctx_lens, H, KV, hd
         _check_device("paged_decode8", out)
     splits = splits8(B * KV * -(-(H // KV) // 8), width * bs if max_ctx is None else min(width * bs, max_ctx))
     # a workspace of this call's own: the allocator keeps it for the stream's later work, or inside the graph that captures it
-    ws = torch.empty((_bound.get("dlti_paged_decode8_floats") or _bind("dlti_paged_decode8_floats"))(B, H, splits), dtype=torch.float32, device=q.device) if splits > 8 else None
+    ws = None
+    if splits > 8:
+        floats = _bound.get("dlti_paged_decode8_floats") or _bind("dlti_paged_decode8_floats")
+        ws = torch.empty(floats(B, H, splits), dtype=torch.float32, device=q.device)
     f = _bound.get("dlti_paged_decode8") or _bind("dlti_paged_decode8")
     _lib.check(f(q.data_ptr(), ld, kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
                  width, ctx_lens.data_ptr(), B, bs, H, KV, hd, scale, splits, None if ws is None else ws.data_ptr(),

@@ -31,9 +31,7 @@ from .scheduler import Batch, Scheduler
 from .tokenizer import IncrementalDetokenizer
 
 _BUCKETS = [1, 2, 4, 8, 16, 32, 64, 128, 256, 512]
-
-
-GIVEN_ALL, GIVEN_SOME = 1, 2
+GIVEN_ALL, GIVEN_SOME = 1, 2       # rows of a step that are drawn with given numbers: all of them, or those with min-p among others
 
 
 class StepLayout:
@@ -56,8 +54,8 @@ class StepLayout:
         tokens (over all such prompts) are already in the paged cache: pslots[P] = their cache slots,
         pdst[P] / csrc[T - nd] = where prefix tokens / this step's prompt rows sit in the extended
         [prefix | chunk] attention layout, ecu[npf + 1] = its sequence boundaries. nl: rows whose logits are wanted
-        when that is not one per sampled sequence. given: the step brings the random numbers (unif) that its tokens are drawn with, and min-p: 1 = of
-        all rows, 2 = of the rows with min-p among others (GIVEN_ALL, GIVEN_SOME)."""
+        when that is not one per sampled sequence. given: the step brings the random numbers (unif) that its tokens are drawn with, and min-p
+        (0, GIVEN_ALL or GIVEN_SOME)."""
         ns = npf if ns is None else ns
         self.T, self.nd, self.npf, self.mb, self.ns, self.P = T, nd, npf, mb, ns, P
         B = nd + ns
